@@ -269,6 +269,41 @@ int b200pa_reshape_and_cache(const b200pa_cache_args* args, void* stream);
 int b200pa_reshape_and_cache_flash(const b200pa_cache_args* args, void* stream);
 
 /*
+ * reshape_and_cache / reshape_and_cache_flash with the rotation of queries and keys by their positions on
+ * the way (what a rotation of q and k in place and the KV write behind it do in two launches; no counterpart
+ * in the reference's paged-attention ops).  The arithmetic is fp32, rounded once: to the query's type for
+ * query_out and 16/32-bit caches, to the code of k / k_scale for fp8 caches.
+ *   query_out, query  [num_tokens, num_heads, head_size], row strides query_out_stride / query_stride; the
+ *                     same tensor (pointer and stride) for a rotation in place, else without overlap
+ *   positions         [num_tokens] int64
+ *   cos_sin           [max_position, rot_dim] contiguous: cosines of rot_dim / 2 pairs, then their sines;
+ *                     float32 or of the query's type (table_dtype)
+ *   neighbours        0: pairs (d, d + rot_dim / 2); else (2 d, 2 d + 1).  Dimensions from rot_dim on are copied.
+ * `args`: as for the KV write; its num_tokens counts, rows behind are not touched.  Padded tokens (slot < 0):
+ * only their query is rotated.  A position outside the table reads nothing; what it would have rotated
+ * becomes NaN.
+ */
+typedef struct b200pa_rotary_args {
+  void* query_out;
+  const void* query;
+  const int64_t* positions;
+  const void* cos_sin;
+
+  int64_t query_out_stride;
+  int64_t query_stride;
+  int64_t max_position;
+
+  int32_t num_heads;
+  int32_t rot_dim;
+  int32_t neighbours;
+  int32_t table_dtype; /* b200pa_dtype */
+} b200pa_rotary_args;
+
+int b200pa_rotary_reshape_and_cache(const b200pa_rotary_args* rotary, const b200pa_cache_args* args, void* stream);
+int b200pa_rotary_reshape_and_cache_flash(const b200pa_rotary_args* rotary, const b200pa_cache_args* args,
+                                          void* stream);
+
+/*
  * One layer of an engine step in one call: the KV write of the step's tokens (b200pa_reshape_and_cache;
  * `write` NULL: none), then attention on the same stream, which then starts under the write and waits for
  * it where it first reads the cache.

@@ -167,6 +167,65 @@ def reshape_and_cache_flash(
         key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale)
 
 
+def rotary_reshape_and_cache(
+    query_out: torch.Tensor,
+    positions: torch.Tensor,
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    cos_sin_cache: torch.Tensor,
+    is_neox: bool,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    kv_cache_dtype: str,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+) -> None:
+    """``reshape_and_cache`` with the rotation of queries and keys on the way, in one launch:
+    `query_out` becomes the rotated `query` (the same tensor for a rotation in place; else they must
+    not overlap), the rotated `key` and `value` go to the cache, `key` itself stays as it is.
+
+    `positions` [tokens] int64; `cos_sin_cache` [positions, rot_dim], float32 or of the query's type:
+    cosines of the pairs, then their sines; pairs are (d, d + rot_dim / 2), or neighbours where
+    `is_neox` is false; dimensions from rot_dim on are copied.  ``slot_mapping.numel()`` tokens
+    count, those with a slot below 0 have only their query rotated.  fp32 arithmetic, rounded once:
+    keys of an fp8 cache are quantised from fp32.  What a position outside the table would have
+    rotated becomes NaN."""
+    if not _compiling() and _direct.rotary_reshape_and_cache(
+            query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache,
+            slot_mapping, kv_cache_dtype, k_scale, v_scale):
+        return
+    _cache_ops.rotary_reshape_and_cache(
+        query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache,
+        slot_mapping, kv_cache_dtype, k_scale, v_scale)
+
+
+def rotary_reshape_and_cache_flash(
+    query_out: torch.Tensor,
+    positions: torch.Tensor,
+    query: torch.Tensor,
+    key: torch.Tensor,
+    value: torch.Tensor,
+    cos_sin_cache: torch.Tensor,
+    is_neox: bool,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    slot_mapping: torch.Tensor,
+    kv_cache_dtype: str,
+    k_scale: torch.Tensor,
+    v_scale: torch.Tensor,
+) -> None:
+    """``rotary_reshape_and_cache`` for the caches of ``reshape_and_cache_flash``."""
+    if not _compiling() and _direct.rotary_reshape_and_cache_flash(
+            query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache,
+            slot_mapping, kv_cache_dtype, k_scale, v_scale):
+        return
+    _cache_ops.rotary_reshape_and_cache_flash(
+        query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache,
+        slot_mapping, kv_cache_dtype, k_scale, v_scale)
+
+
 def convert_fp8(
     output: torch.Tensor, input: torch.Tensor, scale: float = 1.0, kv_dtype: str = "fp8"
 ) -> None:

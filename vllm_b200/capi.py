@@ -23,6 +23,8 @@ EXPORTS = (
     "b200pa_paged_attention_v2_noalloc",
     "b200pa_reshape_and_cache",
     "b200pa_reshape_and_cache_flash",
+    "b200pa_rotary_reshape_and_cache",
+    "b200pa_rotary_reshape_and_cache_flash",
     "b200pa_paged_attention_varlen",
     "b200pa_paged_attention_varlen_supported",
     "b200pa_attention_step",
@@ -68,6 +70,14 @@ class CacheArgs(C.Structure):
     ]
 
 
+class RotaryArgs(C.Structure):
+    _fields_ = [
+        ("query_out", C.c_void_p), ("query", C.c_void_p), ("positions", C.c_void_p), ("cos_sin", C.c_void_p),
+        ("query_out_stride", C.c_int64), ("query_stride", C.c_int64), ("max_position", C.c_int64),
+        ("num_heads", C.c_int32), ("rot_dim", C.c_int32), ("neighbours", C.c_int32), ("table_dtype", C.c_int32),
+    ]
+
+
 _lib = None
 
 
@@ -90,6 +100,8 @@ def lib() -> C.CDLL:
             getattr(l, name).argtypes = [C.POINTER(AttnArgs), C.c_void_p]
         for name in ("b200pa_reshape_and_cache", "b200pa_reshape_and_cache_flash"):
             getattr(l, name).argtypes = [C.POINTER(CacheArgs), C.c_void_p]
+        for name in ("b200pa_rotary_reshape_and_cache", "b200pa_rotary_reshape_and_cache_flash"):
+            getattr(l, name).argtypes = [C.POINTER(RotaryArgs), C.POINTER(CacheArgs), C.c_void_p]
         l.b200pa_convert_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_float, C.c_int32,
                                          C.c_int32, C.c_int32, C.c_void_p]
         l.b200pa_decode_route.argtypes = [C.POINTER(AttnArgs), C.POINTER(C.c_int32)]
@@ -141,6 +153,14 @@ def reshape_and_cache(args: CacheArgs, stream: int = 0) -> None:
 
 def reshape_and_cache_flash(args: CacheArgs, stream: int = 0) -> None:
     check(lib().b200pa_reshape_and_cache_flash(C.byref(args), C.c_void_p(stream)))
+
+
+def rotary_reshape_and_cache(rotary: RotaryArgs, args: CacheArgs, stream: int = 0) -> None:
+    check(lib().b200pa_rotary_reshape_and_cache(C.byref(rotary), C.byref(args), C.c_void_p(stream)))
+
+
+def rotary_reshape_and_cache_flash(rotary: RotaryArgs, args: CacheArgs, stream: int = 0) -> None:
+    check(lib().b200pa_rotary_reshape_and_cache_flash(C.byref(rotary), C.byref(args), C.c_void_p(stream)))
 
 
 def attention_step(write: CacheArgs | None, args: AttnArgs, query_start_loc: int, num_tokens: int,

@@ -270,12 +270,7 @@ void fill_cache(b200pa_cache_args& a, torch::Tensor& key, torch::Tensor& value,
   a.head_size = static_cast<int32_t>(key.size(2));
 }
 
-void reshape_and_cache(torch::Tensor& key, torch::Tensor& value, torch::Tensor& key_cache,
-                       torch::Tensor& value_cache, torch::Tensor& slot_mapping,
-                       const std::string& kv_cache_dtype, torch::Tensor& k_scale,
-                       torch::Tensor& v_scale) {
-  b200pa_cache_args a;
-  fill_cache(a, key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale);
+void fill_x(b200pa_cache_args& a, const torch::Tensor& key_cache, const torch::Tensor& value_cache) {
   TORCH_CHECK(key_cache.dim() == 5 && value_cache.dim() == 4,
               "key_cache must be [num_blocks, num_heads, head_size/x, block_size, x] and "
               "value_cache [num_blocks, num_heads, head_size, block_size]");
@@ -283,16 +278,20 @@ void reshape_and_cache(torch::Tensor& key, torch::Tensor& value, torch::Tensor& 
               "reshape_and_cache needs contiguous caches");
   a.block_size = static_cast<int32_t>(key_cache.size(3));
   a.x = static_cast<int32_t>(key_cache.size(4));
+}
+
+void reshape_and_cache(torch::Tensor& key, torch::Tensor& value, torch::Tensor& key_cache,
+                       torch::Tensor& value_cache, torch::Tensor& slot_mapping,
+                       const std::string& kv_cache_dtype, torch::Tensor& k_scale,
+                       torch::Tensor& v_scale) {
+  b200pa_cache_args a;
+  fill_cache(a, key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale);
+  fill_x(a, key_cache, value_cache);
   const at::cuda::OptionalCUDAGuard device_guard(device_of(key));
   check_rc(b200pa_reshape_and_cache(&a, at::cuda::getCurrentCUDAStream().stream()));
 }
 
-void reshape_and_cache_flash(torch::Tensor& key, torch::Tensor& value, torch::Tensor& key_cache,
-                             torch::Tensor& value_cache, torch::Tensor& slot_mapping,
-                             const std::string& kv_cache_dtype, torch::Tensor& k_scale,
-                             torch::Tensor& v_scale) {
-  b200pa_cache_args a;
-  fill_cache(a, key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale);
+void fill_flash(b200pa_cache_args& a, const torch::Tensor& key_cache, const torch::Tensor& value_cache) {
   TORCH_CHECK(key_cache.dim() == 4 && value_cache.dim() == 4,
               "caches must be [num_blocks, block_size, num_heads, head_size] (possibly strided)");
   TORCH_CHECK(key_cache.stride(0) == value_cache.stride(0));
@@ -302,8 +301,92 @@ void reshape_and_cache_flash(torch::Tensor& key, torch::Tensor& value, torch::Te
   a.block_stride = key_cache.stride(0);
   a.page_stride = key_cache.stride(1);
   a.head_stride = key_cache.stride(2);
+}
+
+void reshape_and_cache_flash(torch::Tensor& key, torch::Tensor& value, torch::Tensor& key_cache,
+                             torch::Tensor& value_cache, torch::Tensor& slot_mapping,
+                             const std::string& kv_cache_dtype, torch::Tensor& k_scale,
+                             torch::Tensor& v_scale) {
+  b200pa_cache_args a;
+  fill_cache(a, key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale);
+  fill_flash(a, key_cache, value_cache);
   const at::cuda::OptionalCUDAGuard device_guard(device_of(key));
   check_rc(b200pa_reshape_and_cache_flash(&a, at::cuda::getCurrentCUDAStream().stream()));
+}
+
+// The KV write with the rotation of queries and keys on the way (not an op of the reference; see
+// b200pa_rotary_reshape_and_cache).
+void rotary_write(torch::Tensor& query_out, torch::Tensor& positions, torch::Tensor& query, torch::Tensor& key,
+                  torch::Tensor& value, torch::Tensor& cos_sin_cache, bool is_neox, torch::Tensor& key_cache,
+                  torch::Tensor& value_cache, torch::Tensor& slot_mapping, const std::string& kv_cache_dtype,
+                  torch::Tensor& k_scale, torch::Tensor& v_scale, bool flash) {
+  b200pa_cache_args a;
+  fill_cache(a, key, value, key_cache, value_cache, slot_mapping, kv_cache_dtype, k_scale, v_scale);
+  if (flash) fill_flash(a, key_cache, value_cache);
+  else fill_x(a, key_cache, value_cache);
+  check_cuda(query_out, "query_out");
+  check_cuda(query, "query");
+  check_cuda(positions, "positions");
+  check_cuda(cos_sin_cache, "cos_sin_cache");
+  const int64_t n = slot_mapping.size(0), H = query.dim() == 3 ? query.size(1) : 0, D = key.size(2);
+  auto rows = [&](const torch::Tensor& t, const char* name, int64_t heads) {
+    TORCH_CHECK(t.dim() == 3 && t.size(0) >= n && t.size(1) == heads && t.size(2) == D && t.scalar_type() == key.scalar_type(),
+                name, " must be [tokens, heads, head_size] of the key's type, with a row for every slot");
+    TORCH_CHECK(t.stride(2) == 1 && (heads == 1 || t.stride(1) == D), name, " heads must be contiguous");
+  };
+  rows(query, "query", H);
+  rows(query_out, "query_out", H);
+  TORCH_CHECK(n <= 1 || query_out.stride(0) >= H * D, "the rows of query_out must not overlap");
+  rows(key, "key", key.size(1));
+  rows(value, "value", key.size(1));
+  TORCH_CHECK(slot_mapping.dim() == 1, "slot_mapping must be [tokens]");
+  TORCH_CHECK(positions.scalar_type() == at::ScalarType::Long && positions.is_contiguous() && positions.dim() == 1 &&
+                  positions.size(0) >= n,
+              "positions must be a contiguous int64 tensor [tokens]");
+  TORCH_CHECK(cos_sin_cache.dim() == 2 && cos_sin_cache.is_contiguous() &&
+                  (cos_sin_cache.scalar_type() == at::ScalarType::Float || cos_sin_cache.scalar_type() == key.scalar_type()),
+              "cos_sin_cache must be a contiguous tensor [positions, rot_dim], float32 or of the key's type");
+  TORCH_CHECK(cos_sin_cache.size(1) > 0 && cos_sin_cache.size(1) <= D && cos_sin_cache.size(1) % 2 == 0, "rot_dim ",
+              cos_sin_cache.size(1), " has to be even and at most the head size ", D);
+  const int64_t cache_heads = flash ? key_cache.size(2) : key_cache.size(1);
+  const int64_t cache_dim = flash ? key_cache.size(3) : key_cache.size(2) * key_cache.size(4);
+  TORCH_CHECK(cache_heads == key.size(1) && cache_dim == D && value_cache.numel() == key_cache.numel(),
+              "the caches do not have the key's heads and head size");
+  for (const torch::Tensor* t : {&query_out, &positions, &query, &value, &cos_sin_cache, &key_cache, &value_cache, &slot_mapping})
+    TORCH_CHECK(t->device() == key.device(), "all tensors must be on one device");
+  b200pa_rotary_args r;
+  std::memset(&r, 0, sizeof(r));
+  r.query_out = query_out.data_ptr();
+  r.query = query.data_ptr();
+  r.positions = positions.data_ptr<int64_t>();
+  r.cos_sin = cos_sin_cache.data_ptr();
+  r.query_out_stride = query_out.stride(0);
+  r.query_stride = query.stride(0);
+  r.max_position = cos_sin_cache.size(0);
+  r.num_heads = static_cast<int32_t>(H);
+  r.rot_dim = static_cast<int32_t>(cos_sin_cache.size(1));
+  r.neighbours = is_neox ? 0 : 1;
+  r.table_dtype = dtype_code(cos_sin_cache.scalar_type(), "cos_sin_cache");
+  const at::cuda::OptionalCUDAGuard device_guard(device_of(key));
+  void* stream = at::cuda::getCurrentCUDAStream().stream();
+  check_rc(flash ? b200pa_rotary_reshape_and_cache_flash(&r, &a, stream) : b200pa_rotary_reshape_and_cache(&r, &a, stream));
+}
+
+void rotary_reshape_and_cache(torch::Tensor& query_out, torch::Tensor& positions, torch::Tensor& query,
+                              torch::Tensor& key, torch::Tensor& value, torch::Tensor& cos_sin_cache, bool is_neox,
+                              torch::Tensor& key_cache, torch::Tensor& value_cache, torch::Tensor& slot_mapping,
+                              const std::string& kv_cache_dtype, torch::Tensor& k_scale, torch::Tensor& v_scale) {
+  rotary_write(query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache, slot_mapping,
+               kv_cache_dtype, k_scale, v_scale, false);
+}
+
+void rotary_reshape_and_cache_flash(torch::Tensor& query_out, torch::Tensor& positions, torch::Tensor& query,
+                                    torch::Tensor& key, torch::Tensor& value, torch::Tensor& cos_sin_cache,
+                                    bool is_neox, torch::Tensor& key_cache, torch::Tensor& value_cache,
+                                    torch::Tensor& slot_mapping, const std::string& kv_cache_dtype,
+                                    torch::Tensor& k_scale, torch::Tensor& v_scale) {
+  rotary_write(query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache, value_cache, slot_mapping,
+               kv_cache_dtype, k_scale, v_scale, true);
 }
 
 void convert_fp8(torch::Tensor& dst_cache, torch::Tensor& src_cache, const double scale,
@@ -514,6 +597,19 @@ TORCH_LIBRARY(_C_b200_cache_ops, cache_ops) {
   cache_ops.impl("convert_fp8", torch::kCUDA, &convert_fp8);
 }
 
+TORCH_LIBRARY_FRAGMENT(_C_b200_cache_ops, cache_ops) {
+  cache_ops.def(
+      "rotary_reshape_and_cache(Tensor! query_out, Tensor positions, Tensor query, Tensor key, Tensor value,"
+      " Tensor cos_sin_cache, bool is_neox, Tensor! key_cache, Tensor! value_cache, Tensor slot_mapping,"
+      " str kv_cache_dtype, Tensor k_scale, Tensor v_scale) -> ()");
+  cache_ops.impl("rotary_reshape_and_cache", torch::kCUDA, &rotary_reshape_and_cache);
+  cache_ops.def(
+      "rotary_reshape_and_cache_flash(Tensor! query_out, Tensor positions, Tensor query, Tensor key, Tensor value,"
+      " Tensor cos_sin_cache, bool is_neox, Tensor! key_cache, Tensor! value_cache, Tensor slot_mapping,"
+      " str kv_cache_dtype, Tensor k_scale, Tensor v_scale) -> ()");
+  cache_ops.impl("rotary_reshape_and_cache_flash", torch::kCUDA, &rotary_reshape_and_cache_flash);
+}
+
 // The reference's own operator names (_C / _C_cache_ops) are claimed on request only, never
 // while this library loads: if they were defined here first, a vLLM `_C` extension imported
 // afterwards would fail on the duplicate definitions.  A stand-alone user (the reference's
@@ -704,6 +800,22 @@ PyObject* py_write(PyObject* const* a, Py_ssize_t n, bool flash) {
 PyObject* py_write_x(PyObject*, PyObject* const* a, Py_ssize_t n) { return py_write(a, n, false); }
 PyObject* py_write_flash(PyObject*, PyObject* const* a, Py_ssize_t n) { return py_write(a, n, true); }
 
+PyObject* py_rotary(PyObject* const* a, Py_ssize_t n, bool flash) {
+  if (!plain_state()) Py_RETURN_FALSE;
+  Args in{a, n};
+  at::Tensor out = in.tensor(), pos = in.tensor(), q = in.tensor(), k = in.tensor(), v = in.tensor(), table = in.tensor();
+  const int64_t neox = in.integer();
+  at::Tensor kc = in.tensor(), vc = in.tensor(), slots = in.tensor();
+  const std::string kv = in.text();
+  at::Tensor ks = in.tensor(), vs = in.tensor();
+  return direct(in, [&] {
+    rotary_write(out, pos, q, k, v, table, neox != 0, kc, vc, slots, kv, ks, vs, flash);
+    return true;
+  });
+}
+PyObject* py_rotary_x(PyObject*, PyObject* const* a, Py_ssize_t n) { return py_rotary(a, n, false); }
+PyObject* py_rotary_flash(PyObject*, PyObject* const* a, Py_ssize_t n) { return py_rotary(a, n, true); }
+
 // One attention layer of an engine step: KV write, then attention, straight from the tensors that
 // the engine hands over (no views, no copies, no scratch tensors where the library's workspace does).
 PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -841,6 +953,10 @@ PyMethodDef kMethods[] = {
     {"reshape_and_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_write_x)), METH_FASTCALL,
      nullptr},
     {"reshape_and_cache_flash", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_write_flash)),
+     METH_FASTCALL, nullptr},
+    {"rotary_reshape_and_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_rotary_x)), METH_FASTCALL,
+     nullptr},
+    {"rotary_reshape_and_cache_flash", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_rotary_flash)),
      METH_FASTCALL, nullptr},
     {"attention_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_step)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
