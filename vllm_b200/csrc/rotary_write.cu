@@ -9,7 +9,10 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "decode_common.cuh"
 #include "kv_quant.cuh"
+#include "kv_write_windows.h"
+#include "launch_state.cuh"
 
 namespace b200pa {
 
@@ -100,9 +103,354 @@ __global__ void __launch_bounds__(256) rotary_write_plain_kernel(const RotaryPar
   }
 }
 
+// How a launch of the kernel below is divided.
+struct RotaryPlan {
+  int units;                       // of a head: pairs of 16-byte chunks that are rotated together, then chunks
+  int tokens, lanes;               // tokens of a block; heads that its threads work on at once (Q, K, flash V)
+  int q_heads, q_parts, q_blocks;  // heads of a block, parts that they make, blocks
+  int k_heads, k_parts, k_blocks;  // ... of K; in the flash layout V as well
+  int v_heads, v_parts, v_blocks;  // V of the x-layout: tiles of 16 tokens
+  int v_dims;                      // head dimensions of a warp's item there
+  bool few;                        // less than a wave of blocks
+};
+
+constexpr int kRotaryThreads = 256;
+constexpr int kRotaryPitch = 64 * 2 + 16;  // bytes between two token rows of a transposed tile
+
+template <typename in_t>
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (std::is_same_v<in_t, __nv_bfloat16>) {
+      f[2 * i] = __uint_as_float(w[i] << 16);
+      f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    } else {
+      const float2 t = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+      f[2 * i] = t.x;
+      f[2 * i + 1] = t.y;
+    }
+  }
+}
+template <typename in_t>
+__device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
+  constexpr bool kBf = std::is_same_v<in_t, __nv_bfloat16>;
+  return make_uint4(pack2<kBf>(f[0], f[1]), pack2<kBf>(f[2], f[3]), pack2<kBf>(f[4], f[5]), pack2<kBf>(f[6], f[7]));
+}
+
+// 16-bit tensors, everything in chunks of 8 elements.  What bounds it: HBM for prefill steps, of whose bytes the
+// queries are most; a chain of trips to memory (position -> table, slot -> store) for decode steps.  Blocks of one
+// launch do different things:
+//   * Q, K and V of the flash layout: a thread owns one unit of a head (the two chunks that a rotation of halves
+//     combines, or one chunk) of one token, loads its cosines and sines once and walks over heads, four at a time;
+//   * V of the x-layout is a transpose: a warp takes 16 tokens x up to 64 dimensions of a head through shared
+//     memory (ldmatrix.trans gives a lane four tokens of a dimension).  Tiles are moved onto 16-slot boundaries of
+//     the cache as in the other KV write kernels (kv_write_windows.h).
+template <typename in_t, int KV, bool kHalves>
+__global__ void __launch_bounds__(kRotaryThreads, 3) rotary_write_kernel(const RotaryParams p, const RotaryPlan plan) {
+  using cache_t = std::conditional_t<KV == kKvAuto, in_t, uint8_t>;
+  constexpr int E = sizeof(cache_t), HU = 4;
+  __shared__ __align__(16) unsigned char s_tile[kRotaryThreads / 32][16 * kRotaryPitch];
+  const int tid = threadIdx.x;
+  const int D = p.head_size, HK = p.num_kv_heads, B = p.block_size, N = p.num_tokens;
+  if (plan.few) grid_dependency();  // (with more blocks the next grid's would take the places of this one's)
+  else grid_dependency_wait();
+
+  int b = blockIdx.x;
+  if (b < plan.v_blocks) {
+    // ================================================= V of the x-layout
+    const int lane = tid & 31, warp = tid >> 5;
+    const int tile = b / plan.v_parts, h0 = (b - tile * plan.v_parts) * plan.v_heads, h1 = min(HK, h0 + plan.v_heads);
+    const int t0 = tile * 16;
+    auto slot_at = [&](int tok) -> int64_t { return tok >= 0 && tok < N ? __ldg(p.slots + tok) : int64_t(-1); };
+    const int64_t now = slot_at(t0 + lane);
+    int d = 0, before = 0, after = 0;
+    if (B % 16 == 0) {
+      const int64_t back = lane < 3 ? slot_at(t0 - 16 + (lane == 0 ? 0 : lane == 1 ? 8 : 15)) : int64_t(-1);
+      auto from = [&](int64_t v, int l) { return __shfl_sync(0xffffffffu, v, l); };
+      d = tile_shift(from(now, 0), from(now, 8), from(now, 15));
+      before = tile_shift(from(back, 0), from(back, 1), from(back, 2));
+      after = tile_shift(from(now, 16), from(now, 24), from(now, 31));
+    }
+    const ScaledDiv div(KV == kKvAuto ? 1.f : *p.v_scale);
+    const int DG = plan.v_dims, groups = (D + DG - 1) / DG, items = (h1 - h0) * groups;
+    unsigned char* mine = s_tile[warp];
+    auto window = [&](const TileWindow& w, int64_t slot) {  // slot: of row `lane` (lanes 0 .. 15)
+      if (w.lo >= w.hi) return;
+      const int64_t own = lane >= w.lo && lane < w.hi ? slot : int64_t(-1);
+      const int j = lane & 3;
+      int64_t at[4];  // element of (head 0, this lane's dimension 0) of tokens 4 j .. 4 j + 3
+      bool have[4], quad = B % 4 == 0;
+      int64_t first = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int64_t s = __shfl_sync(0xffffffffu, own, 4 * j + k);
+        if (k == 0) first = s;
+        have[k] = s >= 0;
+        quad = quad && have[k] && s == first + k;
+        const int64_t blk = have[k] ? s / B : 0;
+        at[k] = blk * HK * int64_t(D) * B + (have[k] ? int(s - blk * B) : 0) + int64_t(lane >> 2) * B;
+      }
+      quad = quad && (first & 3) == 0;
+      uint4 in[4];
+      auto load = [&](int item) {
+        const int h = h0 + item / groups, d0 = item % groups * DG;
+        const in_t* src = static_cast<const in_t*>(p.value) + int64_t(h) * D + d0 + (lane & 7) * 8;
+        const bool col = (lane & 7) * 8 < min(DG, D - d0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = 4 * i + (lane >> 3);
+          if (col && r >= w.lo && r < w.hi) in[i] = *reinterpret_cast<const uint4*>(src + int64_t(w.tok + r) * p.value_stride);
+        }
+      };
+      if (warp < items) load(warp);
+      for (int item = warp; item < items; item += kRotaryThreads / 32) {
+        const int h = h0 + item / groups, d0 = item % groups * DG;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          *reinterpret_cast<uint4*>(mine + (4 * i + (lane >> 3)) * kRotaryPitch + (lane & 7) * 16) = in[i];
+        __syncwarp();
+        if (item + kRotaryThreads / 32 < items) load(item + kRotaryThreads / 32);
+        const int mr = lane & 7, mi = lane >> 3, mtok = (mr >> 1) * 4 + (mr & 1) + (mi & 1) * 2;
+        const uint32_t row = smem_u32(mine) + mtok * kRotaryPitch + (mi >> 1) * 16;
+        const int n16 = min(DG, D - d0) / 16;
+        for (int i16 = 0; i16 < n16; ++i16) {
+          uint32_t r[4];  // (tokens 4j, 4j+1), (4j+2, 4j+3) of row d; the same of row d + 8
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                       : "r"(row + i16 * 32));
+          const int64_t to = (int64_t(h) * D + d0 + i16 * 16) * B;
+          cache_t* base = static_cast<cache_t*>(p.value_cache) + to;
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            uint32_t w2[2] = {r[2 * i], r[2 * i + 1]};
+            if constexpr (KV != kKvAuto) {
+              uint32_t o[1];
+              convert_words<in_t, KV, 2>(w2, o, div);
+              w2[0] = o[0];
+            }
+            if (quad) {
+              cache_t* dst = base + at[0] + 8 * i * B;
+              if constexpr (E == 1) *reinterpret_cast<uint32_t*>(dst) = w2[0];
+              else *reinterpret_cast<uint2*>(dst) = make_uint2(w2[0], w2[1]);
+            } else {
+#pragma unroll
+              for (int k = 0; k < 4; ++k) {
+                if (!have[k]) continue;
+                cache_t* dst = base + at[k] + 8 * i * B;
+                if constexpr (E == 1) *reinterpret_cast<unsigned char*>(dst) = static_cast<unsigned char>(w2[0] >> (8 * k));
+                else *reinterpret_cast<uint16_t*>(dst) = static_cast<uint16_t>(w2[k >> 1] >> (16 * (k & 1)));
+              }
+            }
+          }
+        }
+        __syncwarp();
+      }
+    };
+    const TileWindow own = tile_window(t0, N, d, after), front = tile_front_window(t0, d, before);
+    window(own, __shfl_sync(0xffffffffu, now, (lane + d) & 31));
+    window(front, __shfl_sync(0xffffffffu, now, (lane + d) & 15));
+    return;
+  }
+  b -= plan.v_blocks;
+
+  // ================================================= rows: K (and flash V), then Q
+  const int unit = tid % plan.units, row = tid / plan.units;
+  const int tl = row % plan.tokens, hl = row / plan.tokens;
+  if (hl >= plan.lanes) return;
+  const int rot_units = p.rot / (kHalves ? 16 : 8);
+  const bool turned = unit < rot_units;
+  // dimensions of the unit's chunks
+  const int d0 = kHalves && turned ? unit * 8 : p.rot + (unit - rot_units) * 8;
+  const int d1 = d0 + p.rot / 2;  // (halves only)
+  const bool is_q = b >= plan.k_blocks;
+  const bool is_v = !is_q && p.x == 0 && b >= plan.k_blocks / 2;  // (flash: as many blocks of V as of K)
+  if (is_q) b -= plan.k_blocks;
+  else if (is_v) b -= plan.k_blocks / 2;
+  const int parts = is_q ? plan.q_parts : plan.k_parts, per = is_q ? plan.q_heads : plan.k_heads;
+  const int tile = b / parts;
+  const int h_end = min(is_q ? p.num_heads : HK, (b - tile * parts + 1) * per);
+  const int tok = tile * plan.tokens + tl;
+  int h = (b - tile * parts) * per + hl;
+  if (tok >= N || h >= h_end) return;
+  const in_t* src = is_q ? static_cast<const in_t*>(p.query) + int64_t(tok) * p.query_stride
+                         : is_v ? static_cast<const in_t*>(p.value) + int64_t(tok) * p.value_stride
+                                : static_cast<const in_t*>(p.key) + int64_t(tok) * p.key_stride;
+  const bool rotate = turned && !is_v;
+  const bool two = kHalves && turned;
+  uint4 in[HU][2];
+  auto load = [&](int i, int head) {
+    const in_t* s = src + int64_t(head) * D;
+    in[i][0] = *reinterpret_cast<const uint4*>(s + d0);
+    if (two) in[i][1] = *reinterpret_cast<const uint4*>(s + d1);
+  };
+#pragma unroll
+  for (int i = 0; i < HU; ++i)
+    if (h + i * plan.lanes < h_end) load(i, h + i * plan.lanes);
+  constexpr int NP = kHalves ? 8 : 4;  // pairs of a unit
+  float cosine[NP], sine[NP];
+  if (rotate) {
+    const int64_t pos = p.positions[tok];
+    if (pos < 0 || pos >= p.max_position) {
+#pragma unroll
+      for (int i = 0; i < NP; ++i) cosine[i] = sine[i] = nan_f32();
+    } else if (p.table_f32) {
+      const float* t = static_cast<const float*>(p.table) + pos * p.rot + unit * NP;
+#pragma unroll
+      for (int i = 0; i < NP; i += 4) {
+        *reinterpret_cast<float4*>(cosine + i) = __ldg(reinterpret_cast<const float4*>(t + i));
+        *reinterpret_cast<float4*>(sine + i) = __ldg(reinterpret_cast<const float4*>(t + p.rot / 2 + i));
+      }
+    } else {
+      const in_t* t = static_cast<const in_t*>(p.table) + pos * p.rot + unit * NP;
+      float c8[8], s8[8];
+      if constexpr (kHalves) {
+        unpack8<in_t>(__ldg(reinterpret_cast<const uint4*>(t)), c8);
+        unpack8<in_t>(__ldg(reinterpret_cast<const uint4*>(t + p.rot / 2)), s8);
+      } else {
+        const uint2 c = __ldg(reinterpret_cast<const uint2*>(t)), s = __ldg(reinterpret_cast<const uint2*>(t + p.rot / 2));
+        unpack8<in_t>(make_uint4(c.x, c.y, 0, 0), c8);
+        unpack8<in_t>(make_uint4(s.x, s.y, 0, 0), s8);
+      }
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        cosine[i] = c8[i];
+        sine[i] = s8[i];
+      }
+    }
+  }
+  // where the chunks go: element of head 0, elements between heads
+  int64_t to0, to1, step;
+  if (is_q) {
+    to0 = int64_t(tok) * p.query_out_stride + d0;
+    to1 = to0 + p.rot / 2;
+    step = D;
+  } else {
+    const int64_t slot = __ldg(p.slots + tok);
+    if (slot < 0) return;
+    const int64_t blk = slot / B;
+    const int off = int(slot - blk * B);
+    if (p.x == 0) {
+      to0 = blk * p.block_stride + off * p.page_stride + d0;
+      to1 = to0 + p.rot / 2;
+      step = p.head_stride;
+    } else {
+      constexpr int X = 16 / E;
+      const int64_t base = blk * HK * int64_t(D) * B + off * X;
+      to0 = base + d0 / X * X * B + d0 % X;
+      to1 = base + d1 / X * X * B + d1 % X;
+      step = int64_t(D) * B;
+    }
+  }
+  const ScaledDiv div(KV == kKvAuto || is_q ? 1.f : is_v ? *p.v_scale : *p.k_scale);
+  auto put = [&](const float (&f)[8], int64_t at) {
+    if (is_q) {
+      *reinterpret_cast<uint4*>(static_cast<in_t*>(p.query_out) + at) = pack8<in_t>(f);
+    } else {
+      cache_t* c = static_cast<cache_t*>(is_v ? p.value_cache : p.key_cache) + at;
+      if constexpr (KV == kKvAuto) {
+        *reinterpret_cast<uint4*>(c) = pack8<in_t>(f);
+      } else {
+        __align__(8) uint8_t o[8];
+        convert_n<float, uint8_t, KV, 8>(f, o, div);
+        *reinterpret_cast<uint2*>(c) = *reinterpret_cast<const uint2*>(o);
+      }
+    }
+  };
+  for (; h < h_end; h += HU * plan.lanes) {
+    const int next = h + HU * plan.lanes;
+#pragma unroll
+    for (int i = 0; i < HU; ++i) {
+      const int hi = h + i * plan.lanes;
+      if (hi >= h_end) break;
+      float a[8], bb[8];
+      unpack8<in_t>(in[i][0], a);
+      if (two) unpack8<in_t>(in[i][1], bb);
+      if (rotate) {
+        if constexpr (kHalves) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float x = a[k], y = bb[k];
+            a[k] = fmaf(x, cosine[k], -(y * sine[k]));
+            bb[k] = fmaf(y, cosine[k], x * sine[k]);
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float x = a[2 * k], y = a[2 * k + 1];
+            a[2 * k] = fmaf(x, cosine[k], -(y * sine[k]));
+            a[2 * k + 1] = fmaf(y, cosine[k], x * sine[k]);
+          }
+        }
+      }
+      put(a, to0 + hi * step);
+      if (two) put(bb, to1 + hi * step);
+    }
+    if (next >= h_end) break;
+#pragma unroll
+    for (int i = 0; i < HU; ++i)
+      if (next + i * plan.lanes < h_end) load(i, next + i * plan.lanes);
+  }
+}
+
+// The plan of a call, or false where the kernel above does not take it.
+static bool rotary_plan(const RotaryParams& p, int cache_size, RotaryPlan* plan) {
+  auto al16 = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+  const int D = p.head_size, N = p.num_tokens, HK = p.num_kv_heads, sms = sm_count();
+  if (D % 16 != 0 || D > 512 || p.rot % (p.neighbours ? 8 : 16) != 0) return false;
+  if (!al16(p.query_out) || !al16(p.query) || !al16(p.key) || !al16(p.value) || !al16(p.key_cache) || !al16(p.value_cache) ||
+      !al16(p.table))
+    return false;
+  if (p.query_out_stride % 8 != 0 || p.query_stride % 8 != 0 || p.key_stride % 8 != 0 || p.value_stride % 8 != 0) return false;
+  const bool flash = p.x == 0;
+  if (flash ? p.block_stride % 8 != 0 || p.page_stride % 8 != 0 || p.head_stride % 8 != 0 : p.x != 16 / cache_size) return false;
+  RotaryPlan r{};
+  r.units = p.neighbours ? D / 8 : p.rot / 16 + (D - p.rot) / 8;
+  const int rows = kRotaryThreads / r.units;
+  r.tokens = 1;
+  while (r.tokens * 2 <= rows && r.tokens < N) r.tokens *= 2;
+  r.lanes = rows / r.tokens;
+  const int64_t tiles = (int64_t(N) + r.tokens - 1) / r.tokens;
+  // heads of a block: 8 to a thread, fewer while that leaves SMs without blocks
+  auto divide = [&](int heads, int& per, int& parts) -> int64_t {
+    per = std::min(heads, 8 * r.lanes);
+    while (per > r.lanes && tiles * ((heads + per - 1) / per) < 4 * sms) per = std::max(r.lanes, per / 2);
+    parts = (heads + per - 1) / per;
+    return tiles * parts;
+  };
+  const int64_t q = divide(p.num_heads, r.q_heads, r.q_parts), k = divide(HK, r.k_heads, r.k_parts) * (flash ? 2 : 1);
+  int64_t v = 0;
+  if (!flash) {
+    const int64_t tiles16 = (int64_t(N) + 15) / 16;
+    r.v_dims = 64;
+    r.v_heads = HK;
+    while (r.v_heads > 1 && tiles16 * ((HK + r.v_heads - 1) / r.v_heads) < 2 * sms) r.v_heads = (r.v_heads + 1) / 2;
+    r.v_parts = (HK + r.v_heads - 1) / r.v_heads;
+    v = tiles16 * r.v_parts;
+    if (v < 2 * sms && r.v_heads == 1) r.v_dims = 16;  // an item to each warp
+  }
+  if (q + k + v > INT32_MAX) return false;
+  r.q_blocks = int(q);
+  r.k_blocks = int(k);
+  r.v_blocks = int(v);
+  r.few = q + k + v <= 3 * int64_t(sms);
+  *plan = r;
+  return true;
+}
+
 template <typename in_t, typename cache_t, int KV>
 static int launch_rotary(const RotaryParams& p, cudaStream_t stream) {
-  const cudaError_t e = launch_dependent(rotary_write_plain_kernel<in_t, cache_t, KV>, dim3(p.num_tokens), dim3(256), 0, stream, p);
+  cudaError_t e = cudaErrorInvalidValue;
+  bool taken = false;
+  if constexpr (sizeof(in_t) == 2) {
+    RotaryPlan plan;
+    taken = rotary_plan(p, sizeof(cache_t), &plan);
+    if (taken)
+      e = launch_dependent(p.neighbours ? rotary_write_kernel<in_t, KV, false> : rotary_write_kernel<in_t, KV, true>,
+                           dim3(plan.q_blocks + plan.k_blocks + plan.v_blocks), dim3(kRotaryThreads), 0, stream, p, plan);
+  }
+  if (!taken)
+    e = launch_dependent(rotary_write_plain_kernel<in_t, cache_t, KV>, dim3(p.num_tokens), dim3(256), 0, stream, p);
   count_launch();
   if (e != cudaSuccess) {
     set_error("rotary KV write kernel launch failed: %s", cudaGetErrorString(e));
