@@ -23,6 +23,8 @@ EXPORTS = (
     "b200pa_paged_attention_v2_noalloc",
     "b200pa_reshape_and_cache",
     "b200pa_reshape_and_cache_flash",
+    "b200pa_paged_attention_shared_prefix",
+    "b200pa_shared_prefix_scratch_bytes",
     "b200pa_rotary_reshape_and_cache",
     "b200pa_rotary_reshape_and_cache_flash",
     "b200pa_paged_attention_varlen",
@@ -102,6 +104,10 @@ def lib() -> C.CDLL:
             getattr(l, name).argtypes = [C.POINTER(CacheArgs), C.c_void_p]
         for name in ("b200pa_rotary_reshape_and_cache", "b200pa_rotary_reshape_and_cache_flash"):
             getattr(l, name).argtypes = [C.POINTER(RotaryArgs), C.POINTER(CacheArgs), C.c_void_p]
+        l.b200pa_paged_attention_shared_prefix.argtypes = [C.POINTER(AttnArgs), C.c_int32, C.c_void_p, C.c_int64,
+                                                           C.c_void_p]
+        l.b200pa_shared_prefix_scratch_bytes.argtypes = [C.POINTER(AttnArgs), C.c_int32]
+        l.b200pa_shared_prefix_scratch_bytes.restype = C.c_int64
         l.b200pa_convert_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_float, C.c_int32,
                                          C.c_int32, C.c_int32, C.c_void_p]
         l.b200pa_decode_route.argtypes = [C.POINTER(AttnArgs), C.POINTER(C.c_int32)]
@@ -153,6 +159,18 @@ def reshape_and_cache(args: CacheArgs, stream: int = 0) -> None:
 
 def reshape_and_cache_flash(args: CacheArgs, stream: int = 0) -> None:
     check(lib().b200pa_reshape_and_cache_flash(C.byref(args), C.c_void_p(stream)))
+
+
+def shared_prefix_scratch_bytes(args: AttnArgs, prefix_len: int) -> int:
+    n = lib().b200pa_shared_prefix_scratch_bytes(C.byref(args), prefix_len)
+    check(min(n, 0))
+    return n
+
+
+def paged_attention_shared_prefix(args: AttnArgs, prefix_len: int, scratch: int, scratch_bytes: int,
+                                  stream: int = 0) -> None:
+    check(lib().b200pa_paged_attention_shared_prefix(C.byref(args), prefix_len, C.c_void_p(scratch), scratch_bytes,
+                                                     C.c_void_p(stream)))
 
 
 def rotary_reshape_and_cache(rotary: RotaryArgs, args: CacheArgs, stream: int = 0) -> None:

@@ -89,10 +89,23 @@ struct DirectShape {
   static constexpr int kResident = D == 32 && GP == 1 ? 4 : kMinCtas;
 };
 
-// grid.x = (sequence, kv head, head group) items x cluster size.
-template <typename QT, int KV, int D, int GP>
-__global__ void __launch_bounds__(kDirectWarps * 32, DirectShape<KV, D, GP>::kMinCtas)
-pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
+// What the launch in front has of a prefix that all sequences share (shared_prefix_kernel.cuh): which part of
+// it covers what, for the kernel that has the sequences' own tokens and adds the prefix to them.
+struct SharedPrefixParts {
+  const unsigned char* parts;
+  int prefix_len;
+  int tokens;     // sequences of a row tile
+  int groups;     // of row tiles of a kv head
+  int key_tiles;
+  int cut;        // key tiles of a CTA
+  int tiles;      // row tiles of a group that a slot holds: 2, or 1
+  int turns;      // 1: a slot's two tiles are parts of the same rows
+};
+
+// grid.x = (sequence, kv head, head group) items x cluster size.  kBehind: attends to what a sequence has behind the
+// shared prefix, and adds the prefix's parts.
+template <typename QT, int KV, int D, int GP, bool kBehind>
+__device__ __forceinline__ void decode_direct(const DecodeParams& p, const int cluster, const SharedPrefixParts& pre) {
   using TR = DecodeTraits<QT, KV, D, GP>;
   using SH = DirectShape<KV, D, GP>;
   constexpr bool kFp8 = TR::kFp8;
@@ -122,9 +135,10 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
   const int hq0 = kvh * p.group + hg * HEADS;
   const int nheads = min(HEADS, p.group - hg * HEADS);
   const int B = p.block_size, b_shift = 31 - __clz(B);
-  if (!p.early) grid_dependency();
+  // (kBehind: the prefix's kernel lets this one in when all before it is complete, and writes nothing but its parts)
+  if (!kBehind && !p.early) grid_dependency();
 
-  const int len = min(max(__ldcg(p.seq_lens + seq), 0), p.len_cap);
+  const int len = kBehind ? max(__ldcg(p.seq_lens + seq) - pre.prefix_len, 0) : min(max(__ldcg(p.seq_lens + seq), 0), p.len_cap);
   // ---- Q (B operand; n = head g): 16 bytes of K's chunk order per chunk of this lane
   uint32_t qf[GP][NI][SPC][2];
 #pragma unroll
@@ -224,7 +238,7 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
     l_run[nt][0] = l_run[nt][1] = 0.f;
   }
   if (t_begin < t_end) load_ids(t_begin);
-  if (p.early) grid_dependency();  // (from here on K and V)
+  if (!kBehind && p.early) grid_dependency();  // (from here on K and V)
   if (t_begin < t_end) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
@@ -291,6 +305,7 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
         mx = fmaxf(mx, m_run[nt][j]);  // finite: every tile holds at least one valid token
         alpha[nt][j] = fast_exp2(m_run[nt][j] - mx);
         m_run[nt][j] = mx;
+        if (kBehind && mx == -INFINITY) mx = alpha[nt][j] = 0.f;  // (logits of -inf: weights of 0, not NaN)
         s[nt][j] = fast_exp2(lo - mx);
         s[nt][2 + j] = fast_exp2(hi - mx);
         l_run[nt][j] = l_run[nt][j] * alpha[nt][j] + (s[nt][j] + s[nt][2 + j]);
@@ -375,14 +390,59 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
   // ---- merges.  A unit is four head dimensions of one head.
   constexpr int UPH = D / 4;
   const float kv_o = kFp8 ? *p.v_scale : 1.f;
+  // (kBehind: a sum that is NaN is not left out)
+  auto counts = [](float l) { return kBehind ? l != 0.f : l > 0.f; };
+  if constexpr (kBehind) grid_dependency();  // (from here on the prefix's parts)
   auto store = [&](int hl, int d, float4 acc, float m, float l) {
+    if constexpr (kBehind) {
+      // the parts of the row's item lie in slots item + CTA, of the CTAs whose ranges meet it
+      const int tile = seq / pre.tokens, row = (seq - tile * pre.tokens) * p.group + hg * HEADS + hl;
+      const int grp = pre.turns ? tile : tile / pre.tiles;
+      const int64_t it = int64_t(kvh) * pre.groups + grp, u0 = it * pre.key_tiles;
+      const int c0 = int(u0 / pre.cut), c1 = int((u0 + pre.key_tiles - 1) / pre.cut);
+      constexpr int64_t kPart = 128 * (D * 4 + 8);
+      const int per = pre.turns ? 2 : 1;  // parts of the row in a slot, one behind the other
+      const unsigned char* part = pre.parts + ((it + c0) * pre.tiles + (pre.turns ? 0 : tile - grp * pre.tiles)) * kPart;
+      const int64_t step = pre.turns ? kPart : pre.tiles * kPart;
+      const int n = (c1 - c0 + 1) * per;
+      for (int k0 = 0; k0 < n; k0 += 4) {  // four parts requested at a time
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned char* q = part + min(k0 + k, n - 1) * step;
+          ml[k] = __ldcg(reinterpret_cast<const float2*>(q + 128 * D * 4) + row);
+          v[k] = __ldcg(reinterpret_cast<const float4*>(q) + (d / 4) * 128 + row);
+          if (k0 + k >= n) ml[k] = make_float2(-INFINITY, 0.f);
+        }
+        float m_new = m;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (counts(ml[k].y)) m_new = fmaxf(m_new, ml[k].x);
+        const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new);
+        l *= old;
+        acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+        m = m_new;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if (counts(ml[k].y)) {  // (a part in which the row has no key holds no output)
+            const float f = fast_exp2(ml[k].x - m);
+            l += ml[k].y * f;
+            acc.x += f * v[k].x;
+            acc.y += f * v[k].y;
+            acc.z += f * v[k].z;
+            acc.w += f * v[k].w;
+          }
+        }
+      }
+    }
     const float inv = kv_o * __fdividef(1.f, l + 1e-6f);
     uint2 w;
     w.x = pack2<kOutBf>(acc.x * inv, acc.y * inv);
     w.y = pack2<kOutBf>(acc.z * inv, acc.w * inv);
     *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + hq0 + hl) * D + d) = w;
     if (p.lse != nullptr && d == 0)
-      p.lse[int64_t(hq0 + hl) * p.num_seqs + seq] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      p.lse[int64_t(hq0 + hl) * p.num_seqs + seq] = counts(l) ? (m + log2f(l)) * kLn2 : -INFINITY;
   };
   // the four warps
   for (int u = tid; u < nheads * UPH; u += kDirectWarps * 32) {
@@ -397,7 +457,7 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kDirectWarps; ++w) {
-      if (ml[w].y > 0.f) {  // (a warp without tiles has written no output)
+      if (counts(ml[w].y)) {  // (a warp without tiles has written no output)
         const float f = fast_exp2(ml[w].x - m);
         l += ml[w].y * f;
         const float4 v = *reinterpret_cast<const float4*>(s_part + (w * HEADS + hl) * ROW + d);
@@ -443,7 +503,7 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
       m = m_new;
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
-        if (ml[k].y > 0.f) {
+        if (counts(ml[k].y)) {
           const float f = fast_exp2(ml[k].x - m);
           l += ml[k].y * f;
           acc.x += f * v[k].x;
@@ -457,6 +517,18 @@ pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
   }
   cluster_arrive();  // nobody leaves while its shared memory may be read
   cluster_wait();
+}
+
+template <typename QT, int KV, int D, int GP>
+__global__ void __launch_bounds__(kDirectWarps * 32, DirectShape<KV, D, GP>::kMinCtas)
+pa_decode_direct_kernel(const DecodeParams p, const int cluster) {
+  decode_direct<QT, KV, D, GP, false>(p, cluster, SharedPrefixParts{});
+}
+
+template <typename QT, int KV, int D, int GP>
+__global__ void __launch_bounds__(kDirectWarps * 32, DirectShape<KV, D, GP>::kMinCtas)
+pa_decode_behind_kernel(const DecodeParams p, const SharedPrefixParts pre, const int cluster) {
+  decode_direct<QT, KV, D, GP, true>(p, cluster, pre);
 }
 
 }  // namespace b200pa

@@ -14,10 +14,9 @@ struct DirectKernelInfo {
   int resident;     // that fit in fact
 };
 
-template <typename QT, int KV, int D, int GP>
-cudaError_t direct_launch(const DecodeParams& p, int items, int cluster, cudaStream_t stream) {
-  auto kern = pa_decode_direct_kernel<QT, KV, D, GP>;
-  constexpr int smem = DirectShape<KV, D, GP>::kSmem;
+// Launches `kern` in clusters of `cluster` CTAs, or as many as the device has room for.
+template <auto kern, int smem, typename... Args>
+cudaError_t launch_clusters(int items, int cluster, cudaStream_t stream, const Args&... args) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -57,7 +56,12 @@ cudaError_t direct_launch(const DecodeParams& p, int items, int cluster, cudaStr
   }
   if (cluster > limit) cluster = limit;
   set_clusters(items, cluster);
-  return cudaLaunchKernelEx(&cfg, kern, p, cluster);
+  return cudaLaunchKernelEx(&cfg, kern, args..., cluster);
+}
+
+template <typename QT, int KV, int D, int GP>
+cudaError_t direct_launch(const DecodeParams& p, int items, int cluster, cudaStream_t stream) {
+  return launch_clusters<pa_decode_direct_kernel<QT, KV, D, GP>, DirectShape<KV, D, GP>::kSmem>(items, cluster, stream, p);
 }
 
 template <typename QT, int KV, int D>

@@ -1,0 +1,174 @@
+// Host entry of decode attention over a prefix that all sequences of the batch share.
+#include <algorithm>
+#include <cstdint>
+
+#include "launch_state.cuh"
+#include "shared_prefix_inst.cuh"
+#include "tensor_map.cuh"
+
+namespace b200pa {
+
+struct SharedPrefixPlan {
+  SharedPrefixKernels k;  // k.prefix null: the ordinary kernels
+  int row_tiles = 0, groups = 0, key_tiles = 0, cut = 0, turns = 0, tiles = 0, grid = 0;
+  int64_t bytes = 0;  // of scratch
+};
+
+static SharedPrefixKernels find_shared_prefix(const b200pa_attn_args& a) {
+  const int es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1;
+  auto al = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
+  // (what the two kernels need: 16-byte accesses; strides that a tensor map holds)
+  const bool fits = (a.block_size == 16 || a.block_size == 32) && a.num_heads / a.num_kv_heads <= 128 && al(a.key_cache) &&
+                    al(a.value_cache) && al(a.query) && al(a.out) && (a.kv_block_stride * es) % 16 == 0 &&
+                    (a.kv_head_stride * es) % 16 == 0 &&
+                    (es == 1 || (tensor_map_stride(a.kv_block_stride) && tensor_map_stride(a.kv_head_stride))) &&
+                    a.q_stride % 8 == 0 && tensor_map_stride(a.q_stride) && a.blocksparse_vert_stride <= 1;
+  if (!fits) return {};
+  const int group = a.num_heads / a.num_kv_heads;
+  return a.head_size <= 80    ? find_shared_prefix_small(a.head_size, a.q_dtype, a.kv_dtype, group)
+         : a.head_size <= 112 ? find_shared_prefix_mid(a.head_size, a.q_dtype, a.kv_dtype, group)
+         : a.head_size <= 128 ? find_shared_prefix_128(a.head_size, a.q_dtype, a.kv_dtype, group)
+                              : find_shared_prefix_large(a.head_size, a.q_dtype, a.kv_dtype, group);
+}
+
+static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix_len) {
+  SharedPrefixPlan r;
+  if (a.num_seqs < 2 || prefix_len == 0) return r;
+  const SharedPrefixKernels k = find_shared_prefix(a);
+  if (k.prefix == nullptr) return r;
+  const int sms = sm_count(), group = a.num_heads / a.num_kv_heads, T = 128 / group;
+  r.row_tiles = (a.num_seqs + T - 1) / T;
+  r.turns = k.row_tiles == 2 && r.row_tiles == 1;
+  const int per = r.turns ? 1 : k.row_tiles;
+  r.groups = (r.row_tiles + per - 1) / per;
+  r.tiles = r.turns ? 2 : k.row_tiles;
+  r.key_tiles = (prefix_len + k.keys - 1) / k.keys;
+  const int64_t items = int64_t(a.num_kv_heads) * r.groups, units = items * r.key_tiles;
+  const int64_t behind = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
+  if (units > INT32_MAX / 2 || behind > INT32_MAX / 16) return r;
+  r.cut = int((units + sms - 1) / sms);
+  r.grid = int((units + r.cut - 1) / r.cut);
+  r.bytes = (items + r.grid) * r.tiles * int64_t(k.part_bytes);
+  r.k = k;
+  return r;
+}
+
+static int check_shared_prefix(const b200pa_attn_args* a, int32_t prefix_len) {
+  if (const int bad = attention_check(a, false); bad != B200PA_OK) return bad;
+  B200PA_CHECK_ARG(prefix_len >= 0 && prefix_len % a->block_size == 0,
+                   "prefix_len %d has to be a multiple of the block size %d", prefix_len, a->block_size);
+  B200PA_CHECK_ARG(a->num_seqs == 0 || prefix_len / a->block_size <= a->max_num_blocks_per_seq,
+                   "prefix_len %d does not fit block tables of %d blocks", prefix_len, a->max_num_blocks_per_seq);
+  B200PA_CHECK_ARG(a->blocksparse_vert_stride <= 1, "a shared prefix and block-sparse attention do not go together");
+  return B200PA_OK;
+}
+
+// A dimension of size 1 may come with any stride.
+static b200pa_attn_args with_plain_strides(b200pa_attn_args a) {
+  if (a.num_kv_heads == 1) a.kv_head_stride = int64_t(a.head_size) * a.block_size;
+  if (a.num_seqs == 1) a.q_stride = int64_t(a.num_heads) * a.head_size;
+  return a;
+}
+
+}  // namespace b200pa
+
+extern "C" int64_t b200pa_shared_prefix_scratch_bytes(const b200pa_attn_args* args, int32_t prefix_len) {
+  using namespace b200pa;
+  if (const int bad = check_shared_prefix(args, prefix_len); bad != B200PA_OK) return bad;
+  if (args->num_seqs == 0) return 0;
+  return shared_prefix_plan(with_plain_strides(*args), prefix_len).bytes;
+}
+
+extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args, int32_t prefix_len, void* scratch,
+                                                    int64_t scratch_bytes, void* stream) {
+  using namespace b200pa;
+  if (const int bad = check_shared_prefix(args, prefix_len); bad != B200PA_OK || args->num_seqs == 0) return bad;
+  const b200pa_attn_args plain = with_plain_strides(*args), *a = &plain;
+  const SharedPrefixPlan plan = shared_prefix_plan(*a, prefix_len);
+  if (plan.k.prefix == nullptr) return b200pa_paged_attention_v1(a, stream);
+  B200PA_CHECK_ARG(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0 && scratch_bytes >= plan.bytes,
+                   "a shared prefix needs %lld bytes of scratch on a 16-byte boundary, got %lld", (long long)plan.bytes,
+                   (long long)scratch_bytes);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  SharedPrefixParams p{};
+  p.q = a->query;
+  p.kc = a->key_cache;
+  p.vc = a->value_cache;
+  p.blocks = a->block_tables;
+  p.seq_lens = a->seq_lens;
+  p.alibi = a->alibi_slopes;
+  p.k_scale = a->k_scale;
+  p.parts = static_cast<unsigned char*>(scratch);
+  p.status = device_status_ptr();
+  if (p.status == nullptr) {
+    set_error("could not resolve the device-side status word");
+    return B200PA_ECUDA;
+  }
+  p.q_stride = a->q_stride;
+  p.kv_block_stride = a->kv_block_stride;
+  p.kv_head_stride = a->kv_head_stride;
+  p.num_seqs = a->num_seqs;
+  p.num_kv_heads = a->num_kv_heads;
+  p.group = a->num_heads / a->num_kv_heads;
+  p.block_size = a->block_size;
+  p.prefix_len = prefix_len;
+  p.row_tiles = plan.row_tiles;
+  p.groups = plan.groups;
+  p.key_tiles = plan.key_tiles;
+  p.cut = plan.cut;
+  p.turns = plan.turns;
+  p.scale = a->scale;
+  cudaError_t e = plan.k.prefix(p, a->num_heads, plan.grid, s);
+  count_launch();
+  if (e != cudaSuccess) {
+    set_error("shared prefix kernel launch failed: %s", cudaGetErrorString(e));
+    return B200PA_ECUDA;
+  }
+
+  DecodeParams d{};
+  d.out = a->out;
+  d.q = a->query;
+  d.kc = a->key_cache;
+  d.vc = a->value_cache;
+  d.block_tables = a->block_tables + prefix_len / a->block_size;
+  d.seq_lens = a->seq_lens;
+  d.alibi = a->alibi_slopes;
+  d.k_scale = a->k_scale;
+  d.v_scale = a->v_scale;
+  d.q_stride = a->q_stride;
+  d.kv_block_stride = a->kv_block_stride;
+  d.kv_head_stride = a->kv_head_stride;
+  d.num_seqs = a->num_seqs;
+  d.num_heads = a->num_heads;
+  d.num_kv_heads = a->num_kv_heads;
+  d.block_size = a->block_size;
+  d.max_blocks_per_seq = a->max_num_blocks_per_seq;
+  d.len_cap = INT32_MAX;
+  d.group = p.group;
+  d.head_groups = (p.group + plan.k.heads - 1) / plan.k.heads;
+  d.scale = a->scale;
+  d.lse = a->out_lse;
+  d.status = p.status;
+  SharedPrefixParts pre{};
+  pre.parts = p.parts;
+  pre.prefix_len = prefix_len;
+  pre.tokens = 128 / p.group;
+  pre.groups = plan.groups;
+  pre.key_tiles = plan.key_tiles;
+  pre.cut = plan.cut;
+  pre.tiles = plan.tiles;
+  pre.turns = plan.turns;
+  // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
+  const int64_t items = int64_t(d.num_seqs) * d.num_kv_heads * d.head_groups;
+  const int64_t places = int64_t(sm_count()) * plan.k.ctas_per_sm;
+  const int64_t tiles = (int64_t(std::max(a->max_seq_len - prefix_len, 1)) + 15) / 16;
+  int cluster = 1;
+  while (cluster < 8 && items * cluster * 10 <= places * 6 && cluster * kDirectWarps < tiles) cluster *= 2;
+  e = plan.k.behind(d, pre, int(items), cluster, s);
+  count_launch();
+  if (e != cudaSuccess) {
+    set_error("shared prefix decode kernel launch failed: %s", cudaGetErrorString(e));
+    return B200PA_ECUDA;
+  }
+  return B200PA_OK;
+}

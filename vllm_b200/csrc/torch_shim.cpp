@@ -226,6 +226,46 @@ bool paged_attention_varlen(torch::Tensor& out, torch::Tensor& query, torch::Ten
   return true;
 }
 
+// Decode attention over a prefix that the sequences share (not an op of the reference).
+void paged_attention_shared_prefix(torch::Tensor& out, torch::Tensor& query, torch::Tensor& key_cache,
+                                   torch::Tensor& value_cache, int64_t num_kv_heads, double scale,
+                                   torch::Tensor& block_tables, torch::Tensor& seq_lens, int64_t prefix_len,
+                                   int64_t block_size, int64_t max_seq_len,
+                                   const std::optional<torch::Tensor>& alibi_slopes,
+                                   const std::string& kv_cache_dtype, torch::Tensor& k_scale,
+                                   torch::Tensor& v_scale, std::optional<torch::Tensor> lse) {
+  b200pa_attn_args a;
+  fill_attn(a, out, query, key_cache, value_cache, num_kv_heads, scale, block_tables, seq_lens,
+            block_size, max_seq_len, alibi_slopes, kv_cache_dtype, k_scale, v_scale, 0, 0, 0, 64, 0);
+  const int64_t n = query.size(0), D = query.size(2);
+  TORCH_CHECK(out.numel() == query.numel(), "out must have the query's shape");
+  TORCH_CHECK(block_tables.dim() == 2 && block_tables.size(0) >= n && seq_lens.dim() == 1 && seq_lens.size(0) >= n,
+              "block_tables [num_seqs, blocks] and seq_lens [num_seqs] must have a row for every sequence");
+  TORCH_CHECK(key_cache.size(1) == num_kv_heads && key_cache.size(2) * key_cache.size(4) == D &&
+                  key_cache.size(3) == block_size && value_cache.size(1) == num_kv_heads && value_cache.size(2) == D &&
+                  value_cache.size(3) == block_size,
+              "the caches do not have these heads, head size and block size");
+  TORCH_CHECK(prefix_len >= 0 && prefix_len <= INT32_MAX, "prefix_len ", prefix_len, " is out of range");
+  TORCH_CHECK(!alibi_slopes.has_value() || alibi_slopes->numel() == query.size(1), "alibi_slopes must be [num_heads]");
+  const auto dev = query.device();
+  for (const torch::Tensor* t : {&out, &key_cache, &value_cache, &block_tables, &seq_lens})
+    TORCH_CHECK(t->device() == dev, "all tensors must be on one device");
+  if (lse.has_value()) {
+    TORCH_CHECK(lse->device() == dev && lse->scalar_type() == at::ScalarType::Float && lse->is_contiguous() &&
+                    lse->dim() == 2 && lse->size(0) == query.size(1) && lse->size(1) == n,
+                "lse must be a contiguous float32 tensor [num_heads, num_seqs]");
+    a.out_lse = lse->data_ptr<float>();
+  }
+  const at::cuda::OptionalCUDAGuard device_guard(dev);
+  const int64_t bytes = b200pa_shared_prefix_scratch_bytes(&a, static_cast<int32_t>(prefix_len));
+  check_rc(bytes < 0 ? static_cast<int>(bytes) : 0);
+  torch::Tensor scratch;
+  if (bytes > 0) scratch = at::empty({bytes}, query.options().dtype(at::ScalarType::Byte));
+  check_rc(b200pa_paged_attention_shared_prefix(&a, static_cast<int32_t>(prefix_len),
+                                                bytes > 0 ? scratch.data_ptr() : nullptr, bytes,
+                                                at::cuda::getCurrentCUDAStream().stream()));
+}
+
 void fill_cache(b200pa_cache_args& a, torch::Tensor& key, torch::Tensor& value,
                 torch::Tensor& key_cache, torch::Tensor& value_cache, torch::Tensor& slot_mapping,
                 const std::string& kv_cache_dtype, torch::Tensor& k_scale, torch::Tensor& v_scale) {
@@ -584,6 +624,15 @@ TORCH_LIBRARY_FRAGMENT(_C_b200, ops) {
   ops.impl("paged_attention_varlen", torch::kCUDA, &paged_attention_varlen);
 }
 
+TORCH_LIBRARY_FRAGMENT(_C_b200, ops) {
+  ops.def(
+      "paged_attention_shared_prefix(Tensor! out, Tensor query, Tensor key_cache, Tensor value_cache,"
+      " int num_kv_heads, float scale, Tensor block_tables, Tensor seq_lens, int prefix_len, int block_size,"
+      " int max_seq_len, Tensor? alibi_slopes, str kv_cache_dtype, Tensor k_scale, Tensor v_scale,"
+      " Tensor!? lse) -> ()");
+  ops.impl("paged_attention_shared_prefix", torch::kCUDA, &paged_attention_shared_prefix);
+}
+
 TORCH_LIBRARY(_C_b200_cache_ops, cache_ops) {
   cache_ops.def(kSwapSchema);
   cache_ops.impl("swap_blocks", torch::kCUDA, &swap_blocks);
@@ -785,6 +834,24 @@ PyObject* py_paged_attention(PyObject* const* a, Py_ssize_t n, bool v2) {
 PyObject* py_v1(PyObject*, PyObject* const* a, Py_ssize_t n) { return py_paged_attention(a, n, false); }
 PyObject* py_v2(PyObject*, PyObject* const* a, Py_ssize_t n) { return py_paged_attention(a, n, true); }
 
+PyObject* py_shared_prefix(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (!plain_state()) Py_RETURN_FALSE;
+  Args in{a, n};
+  at::Tensor out = in.tensor(), q = in.tensor(), kc = in.tensor(), vc = in.tensor();
+  const int64_t hk = in.integer();
+  const double scale = in.real();
+  at::Tensor bt = in.tensor(), sl = in.tensor();
+  const int64_t prefix = in.integer(), bs = in.integer(), max_len = in.integer();
+  const auto alibi = in.optional_tensor();
+  const std::string kv = in.text();
+  at::Tensor ks = in.tensor(), vs = in.tensor();
+  const auto lse = in.optional_tensor();
+  return direct(in, [&] {
+    paged_attention_shared_prefix(out, q, kc, vc, hk, scale, bt, sl, prefix, bs, max_len, alibi, kv, ks, vs, lse);
+    return true;
+  });
+}
+
 PyObject* py_write(PyObject* const* a, Py_ssize_t n, bool flash) {
   if (!plain_state()) Py_RETURN_FALSE;
   Args in{a, n};
@@ -953,6 +1020,8 @@ PyMethodDef kMethods[] = {
     {"reshape_and_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_write_x)), METH_FASTCALL,
      nullptr},
     {"reshape_and_cache_flash", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_write_flash)),
+     METH_FASTCALL, nullptr},
+    {"paged_attention_shared_prefix", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_shared_prefix)),
      METH_FASTCALL, nullptr},
     {"rotary_reshape_and_cache", reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(py_rotary_x)), METH_FASTCALL,
      nullptr},
