@@ -58,6 +58,40 @@ struct DecodeParams {
   int early;  // 1: the launch in front is the step's KV write, see launch_dependent
 };
 
+// What the launch in front has of a prefix that all sequences share (shared_prefix_kernel.cuh): which part of
+// it covers what, for the kernels that have the sequences' own tokens and add the prefix to them.
+struct SharedPrefixParts {
+  const unsigned char* parts;
+  int prefix_len;
+  int tokens;     // sequences of a row tile
+  int groups;     // of row tiles of a kv head
+  int key_tiles;
+  int cut;        // key tiles of a CTA
+  int tiles;      // row tiles of a group that a slot holds: 2, or 1
+  int turns;      // 1: a slot's two tiles are parts of the same rows
+  // the persistent kernel's own: partials of sequences that are cut (two slots to a range), arrivals at every item
+  // (zeroed by the prefix's kernel)
+  unsigned char* own;
+  unsigned* arrive;
+
+  // The parts of a row (`head`: of its kv head's group) at head size D: the first, bytes between two, how many;
+  // its place in them.  They lie in slots item + CTA, of the CTAs whose ranges meet the row's item.
+  struct Row {
+    const unsigned char* first;
+    int64_t step;
+    int n, row;
+  };
+  template <int D>
+  __device__ __forceinline__ Row row(int seq, int kvh, int head, int group) const {
+    constexpr int64_t kPart = 128 * (D * 4 + 8);
+    const int tile = seq / tokens, grp = turns ? tile : tile / tiles;
+    const int64_t it = int64_t(kvh) * groups + grp, u0 = it * key_tiles;
+    const int c0 = int(u0 / cut), c1 = int((u0 + key_tiles - 1) / cut);
+    return {parts + ((it + c0) * tiles + (turns ? 0 : tile - grp * tiles)) * kPart, turns ? kPart : tiles * kPart,
+            (c1 - c0 + 1) * (turns ? 2 : 1), (seq - tile * tokens) * group + head};
+  }
+};
+
 // ------------------------------------------------------------------ PTX wrappers
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));

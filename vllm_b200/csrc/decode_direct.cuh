@@ -89,19 +89,6 @@ struct DirectShape {
   static constexpr int kResident = D == 32 && GP == 1 ? 4 : kMinCtas;
 };
 
-// What the launch in front has of a prefix that all sequences share (shared_prefix_kernel.cuh): which part of
-// it covers what, for the kernel that has the sequences' own tokens and adds the prefix to them.
-struct SharedPrefixParts {
-  const unsigned char* parts;
-  int prefix_len;
-  int tokens;     // sequences of a row tile
-  int groups;     // of row tiles of a kv head
-  int key_tiles;
-  int cut;        // key tiles of a CTA
-  int tiles;      // row tiles of a group that a slot holds: 2, or 1
-  int turns;      // 1: a slot's two tiles are parts of the same rows
-};
-
 // grid.x = (sequence, kv head, head group) items x cluster size.  kBehind: attends to what a sequence has behind the
 // shared prefix, and adds the prefix's parts.
 template <typename QT, int KV, int D, int GP, bool kBehind>
@@ -394,48 +381,6 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
   auto counts = [](float l) { return kBehind ? l != 0.f : l > 0.f; };
   if constexpr (kBehind) grid_dependency();  // (from here on the prefix's parts)
   auto store = [&](int hl, int d, float4 acc, float m, float l) {
-    if constexpr (kBehind) {
-      // the parts of the row's item lie in slots item + CTA, of the CTAs whose ranges meet it
-      const int tile = seq / pre.tokens, row = (seq - tile * pre.tokens) * p.group + hg * HEADS + hl;
-      const int grp = pre.turns ? tile : tile / pre.tiles;
-      const int64_t it = int64_t(kvh) * pre.groups + grp, u0 = it * pre.key_tiles;
-      const int c0 = int(u0 / pre.cut), c1 = int((u0 + pre.key_tiles - 1) / pre.cut);
-      constexpr int64_t kPart = 128 * (D * 4 + 8);
-      const int per = pre.turns ? 2 : 1;  // parts of the row in a slot, one behind the other
-      const unsigned char* part = pre.parts + ((it + c0) * pre.tiles + (pre.turns ? 0 : tile - grp * pre.tiles)) * kPart;
-      const int64_t step = pre.turns ? kPart : pre.tiles * kPart;
-      const int n = (c1 - c0 + 1) * per;
-      for (int k0 = 0; k0 < n; k0 += 4) {  // four parts requested at a time
-        float2 ml[4];
-        float4 v[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const unsigned char* q = part + min(k0 + k, n - 1) * step;
-          ml[k] = __ldcg(reinterpret_cast<const float2*>(q + 128 * D * 4) + row);
-          v[k] = __ldcg(reinterpret_cast<const float4*>(q) + (d / 4) * 128 + row);
-          if (k0 + k >= n) ml[k] = make_float2(-INFINITY, 0.f);
-        }
-        float m_new = m;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          if (counts(ml[k].y)) m_new = fmaxf(m_new, ml[k].x);
-        const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new);
-        l *= old;
-        acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
-        m = m_new;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if (counts(ml[k].y)) {  // (a part in which the row has no key holds no output)
-            const float f = fast_exp2(ml[k].x - m);
-            l += ml[k].y * f;
-            acc.x += f * v[k].x;
-            acc.y += f * v[k].y;
-            acc.z += f * v[k].z;
-            acc.w += f * v[k].w;
-          }
-        }
-      }
-    }
     const float inv = kv_o * __fdividef(1.f, l + 1e-6f);
     uint2 w;
     w.x = pack2<kOutBf>(acc.x * inv, acc.y * inv);
@@ -443,6 +388,40 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
     *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + hq0 + hl) * D + d) = w;
     if (p.lse != nullptr && d == 0)
       p.lse[int64_t(hq0 + hl) * p.num_seqs + seq] = counts(l) ? (m + log2f(l)) * kLn2 : -INFINITY;
+  };
+  // the prefix's parts of a unit, each CTA of the cluster its share of them
+  auto add_parts = [&](int hl, int d, float4& acc, float& m, float& l) {
+    const SharedPrefixParts::Row r = pre.row<D>(seq, kvh, hg * HEADS + hl, p.group);
+    for (int k0 = rank; k0 < r.n; k0 += 4 * cluster) {  // four parts requested at a time
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const unsigned char* q = r.first + min(k0 + k * cluster, r.n - 1) * r.step;
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(q + 128 * D * 4) + r.row);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(q) + (d / 4) * 128 + r.row);
+        if (k0 + k * cluster >= r.n) ml[k] = make_float2(-INFINITY, 0.f);
+      }
+      float m_new = m;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (counts(ml[k].y)) m_new = fmaxf(m_new, ml[k].x);
+      const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new);
+      l *= old;
+      acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+      m = m_new;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (counts(ml[k].y)) {  // (a part in which the row has no key holds no output)
+          const float f = fast_exp2(ml[k].x - m);
+          l += ml[k].y * f;
+          acc.x += f * v[k].x;
+          acc.y += f * v[k].y;
+          acc.z += f * v[k].z;
+          acc.w += f * v[k].w;
+        }
+      }
+    }
   };
   // the four warps
   for (int u = tid; u < nheads * UPH; u += kDirectWarps * 32) {
@@ -467,6 +446,7 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
         acc.w += f * v.w;
       }
     }
+    if constexpr (kBehind) add_parts(hl, d, acc, m, l);
     if (cluster == 1) {
       store(hl, d, acc, m, l);
     } else {

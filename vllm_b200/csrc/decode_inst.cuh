@@ -23,10 +23,8 @@ constexpr int decode_max_warps() {
   return (D * GP <= 128) ? 16 : (D * GP <= 256 ? 12 : 8);
 }
 
-template <typename QT, int KV, int D, int GP, int NT>
-cudaError_t decode_launch(const DecodeParams& p, int grid, int threads, size_t smem,
-                          cudaStream_t stream) {
-  auto kern = pa_decode_kernel<QT, KV, D, GP, NT, decode_max_warps<KV, D, GP>()>;
+template <auto kern, typename... Args>
+cudaError_t launch_persistent(int grid, int threads, size_t smem, cudaStream_t stream, const Args&... args) {
   // opt in to large dynamic shared memory once per device
   static bool done[64] = {};
   int dev = 0;
@@ -45,7 +43,13 @@ cudaError_t decode_launch(const DecodeParams& p, int grid, int threads, size_t s
     }
     if (dev >= 0 && dev < 64) done[dev] = true;
   }
-  return launch_dependent(kern, dim3(grid), dim3(threads), smem, stream, p);
+  return launch_dependent(kern, dim3(grid), dim3(threads), smem, stream, args...);
+}
+
+template <typename QT, int KV, int D, int GP, int NT>
+cudaError_t decode_launch(const DecodeParams& p, int grid, int threads, size_t smem,
+                          cudaStream_t stream) {
+  return launch_persistent<pa_decode_kernel<QT, KV, D, GP, NT, decode_max_warps<KV, D, GP>()>>(grid, threads, smem, stream, p);
 }
 
 template <typename QT, int KV, int D, int GP>

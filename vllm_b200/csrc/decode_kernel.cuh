@@ -78,9 +78,11 @@ struct DecodeTraits {
 };
 
 // Reads this lane's block id for the 32-page window `win` of an item.
+template <bool kPastL1 = false>
 __device__ __forceinline__ int load_bt(const DecodeParams& p, const WorkItem& it, int win, int lane) {
   const int pg = win * 32 + lane;
   if (pg >= it.npages) return 0;
+  if constexpr (kPastL1) return __ldcg(p.block_tables + int64_t(it.seq) * p.max_blocks_per_seq + it.first_page + pg);
   return __ldg(p.block_tables + int64_t(it.seq) * p.max_blocks_per_seq + it.first_page + pg);
 }
 
@@ -89,6 +91,7 @@ __device__ __forceinline__ int load_bt(const DecodeParams& p, const WorkItem& it
 // partial (kept in the group's first slot), and the warp that completes the last group merges
 // the groups.  One warp merging 60 partials of four heads takes ~14 us, which would be the
 // tail of the launch; groups are merged by different warps as they finish.
+constexpr int kBehindPieces = 32;  // that a sequence is cut into at most, behind a shared prefix
 constexpr int kMergeFan = 8;
 constexpr int kMergeDirectMax = 32;  // (16 measured 2 % slower on a 4-way kv-head shard, equal elsewhere)
 
@@ -520,8 +523,91 @@ __device__ __forceinline__ void merge_partials(float* exp_sums, float* max_logit
   }
 }
 
-template <typename QT, int KV, int D, int GP, int BT, int MAXW>
-__global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodeParams p) {
+// The merge of a sequence that was cut, behind a shared prefix: `np` partials of `nheads` heads and the prefix's parts.
+// (Partials: the first in slot 1 of its range, the others in slot 0 of the ranges behind it, two slots to a range.)  A lane owns four head dimensions (of each 128), four heads at a time; of every source, two at a time,
+// statistics and output are requested together.
+template <typename QT, int D, int HEADS>
+__device__ __noinline__ void merge_behind(const unsigned char* own, int np, const SharedPrefixParts& pre, QT* out,
+                                          int seq, int kvh, int head0, int group, int nheads, int lane, float scale,
+                                          float* lse, int lse_stride) {
+  constexpr bool kOutBf = std::is_same_v<QT, __nv_bfloat16>;
+  constexpr int kSlot = HEADS * (D * 4 + 8);
+  const SharedPrefixParts::Row r = pre.row<D>(seq, kvh, head0, group);
+  const int n = np + r.n;
+  for (int h0 = 0; h0 < nheads; h0 += 4) {
+    const int nh = min(4, nheads - h0);
+    for (int d = lane * 4; d < (D + 127) / 128 * 128; d += 128) {
+      const bool in = d < D;
+      const int dd = in ? d : 0;
+      float4 acc[4];
+      float m[4], l[4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        acc[h] = make_float4(0.f, 0.f, 0.f, 0.f);
+        m[h] = -INFINITY;
+        l[h] = 0.f;
+      }
+      for (int k0 = 0; k0 < n; k0 += 2) {
+        float2 ml[2][4];
+        float4 v[2][4];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const int s = min(k0 + k, n - 1);
+          const unsigned char* q = s < np ? own + (2 * int64_t(s) + (s == 0)) * kSlot : r.first + (s - np) * r.step;
+          const unsigned char* stat = s < np ? q + HEADS * D * 4 + h0 * 8 : q + 128 * D * 4 + (r.row + h0) * 8;
+          const unsigned char* val = s < np ? q + (h0 * D + dd) * 4 : q + (dd * 32 + r.row + h0) * 16;
+          const int step = s < np ? D * 4 : 16;
+#pragma unroll
+          for (int h = 0; h < 4; ++h) {
+            const int hh = h < nh ? h : 0;
+            ml[k][h] = __ldcg(reinterpret_cast<const float2*>(stat + hh * 8));
+            v[k][h] = __ldcg(reinterpret_cast<const float4*>(val + hh * step));
+            if (k0 + k >= n) ml[k][h] = make_float2(-INFINITY, 0.f);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+          float m_new = m[h];
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (ml[k][h].y != 0.f) m_new = fmaxf(m_new, ml[k][h].x);
+          const float old = m_new == -INFINITY ? 0.f : fast_exp2(m[h] - m_new);
+          l[h] *= old;
+          acc[h] = make_float4(acc[h].x * old, acc[h].y * old, acc[h].z * old, acc[h].w * old);
+          m[h] = m_new;
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (ml[k][h].y != 0.f) {  // (what has no key has written no output)
+              const float f = fast_exp2(ml[k][h].x - m_new);
+              l[h] += ml[k][h].y * f;
+              acc[h].x += f * v[k][h].x;
+              acc[h].y += f * v[k][h].y;
+              acc[h].z += f * v[k][h].z;
+              acc[h].w += f * v[k][h].w;
+            }
+          }
+        }
+      }
+#pragma unroll
+      for (int h = 0; h < 4; ++h) {
+        if (h >= nh) break;
+        const float inv = scale * __fdividef(1.f, l[h] + 1e-6f);
+        if (in) {
+          uint2 w;
+          w.x = pack2<kOutBf>(acc[h].x * inv, acc[h].y * inv);
+          w.y = pack2<kOutBf>(acc[h].z * inv, acc[h].w * inv);
+          *reinterpret_cast<uint2*>(out + (h0 + h) * D + d) = w;
+        }
+        if (lse != nullptr && d == 0) lse[int64_t(h0 + h) * lse_stride] = l[h] != 0.f ? (m[h] + log2f(l[h])) * kLn2 : -INFINITY;
+      }
+    }
+  }
+}
+
+// kBehind: attends to what the sequences have behind a shared prefix and adds the prefix's parts (split launches only;
+// partials and arrival counters are in the scratch of the call, partials in fp32).
+template <typename QT, int KV, int D, int GP, int BT, int MAXW, bool kBehind>
+__device__ __forceinline__ void decode_persistent(const DecodeParams& p, const SharedPrefixParts& pre) {
   using TR = DecodeTraits<QT, KV, D, GP>;
   constexpr bool kFp8 = TR::kFp8;
   constexpr bool kBf = TR::kMmaBf16;
@@ -568,8 +654,11 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
   __shared__ int4 s_iter[MAXW];  // per warp: units left, block offset, sequence, head
   __shared__ int4 s_todo[MAXW][2];  // per warp: merges owed (sequence, head item, pieces, piece | level)
   __shared__ int s_ntodo[MAXW];
-  if (!p.early) grid_dependency();
-  const bool flat = p.use_table != 0;
+  // (kBehind: the prefix's kernel lets this one in when all before it is complete; what is read up to the wait for its
+  // parts is read past L1, and by copies of another proxy behind a fence)
+  if (!kBehind && !p.early) grid_dependency();
+  if (kBehind && lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");
+  const bool flat = kBehind || p.use_table != 0;
   const int hsubs = p.num_kv_heads * p.head_groups;
   if (flat) {
     __shared__ int warp_tot[MAXW];
@@ -579,7 +668,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
     const int s0 = min(S, int(threadIdx.x) * per);
     const int s1 = min(S, s0 + per);
     auto units_of = [&](int s) {
-      const int len = min(max(__ldcg(p.seq_lens + s), 0), p.len_cap);
+      const int len = kBehind ? max(__ldcg(p.seq_lens + s) - pre.prefix_len, 0) : min(max(__ldcg(p.seq_lens + s), 0), p.len_cap);
       return max(2, ((len + B - 1) / B + 1) & ~1);
     };
     int mine = 0, mx = 0;
@@ -622,18 +711,19 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
       const long long W = (long long)gridDim.x * nwarps;
       long long C = (U + W - 1) / W;
       C = max(C, (long long)p.min_chunk);
-      C = max(C, (long long)((n_max - 1) / max(1, p.max_partitions - 1) + 1));
+      // (kBehind: any number of slots, but one warp merges them)
+      C = max(C, (long long)((n_max - 1) / (kBehind ? kBehindPieces - 1 : max(1, p.max_partitions - 1)) + 1));
       C = (C + 1) & ~1ll;
       s_plan[0] = int(min(C, (long long)INT32_MAX - 1));
       s_plan[1] = total;
       s_plan[2] = int((U + C - 1) / C);
     }
   }
-  if (p.early) grid_dependency();
+  if (!kBehind && p.early) grid_dependency();
   // The plan reads the lengths past L1 (see launch_dependent); from here on every item of a warp looks its
   // length up again, on the way to its first page.  Without them in L1: 128 sequences of 8192 tokens, 64 / 8
   // heads, fp8, 334 -> 341 us, as a step with its KV write 340 -> 346.
-  if (flat)
+  if (flat && !kBehind)
     for (int s = threadIdx.x; s < p.num_seqs; s += blockDim.x) prefetch_l1(p.seq_lens + s);
   __syncthreads();
 
@@ -733,7 +823,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
     it.hg = hsub % p.head_groups;
     it.tok_end = max(p.seq_lens[it.seq], 0);
     it.npages = (it.tok_end + B - 1) / B;
-    it.bt = load_bt(p, it, 0, lane);
+    it.bt = load_bt<kBehind>(p, it, 0, lane);
     return it;
   };
 
@@ -748,7 +838,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
     const int c0 = cum[st.z];
     const int n = cum[st.z + 1] - c0;      // units of this sequence
     const int take = min(n - st.y, st.x);  // units of it that fall into the range
-    const int len = min(max(p.seq_lens[st.z], 0), p.len_cap);
+    const int len = kBehind ? max(__ldcg(p.seq_lens + st.z) - pre.prefix_len, 0) : min(max(p.seq_lens[st.z], 0), p.len_cap);
     it.seq = st.z;
     it.kvh = st.w / p.head_groups;
     it.hg = st.w % p.head_groups;
@@ -768,7 +858,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
     it.tok_begin = st.y * B;
     it.tok_end = max(it.tok_begin, min(len, (st.y + take) * B));
     it.npages = (it.tok_end - it.tok_begin + B - 1) / B;
-    it.bt = load_bt(p, it, 0, lane);
+    it.bt = load_bt<kBehind>(p, it, 0, lane);
     st.x -= take;
     st.y += take;
     if (st.y == n) {
@@ -852,7 +942,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
       const int win = prod_pg >> 5;
       if (win != pi_win) {
         pi_win = win;
-        pi_bt = load_bt(p, prod_sel ? nxt : cur, win, lane);
+        pi_bt = load_bt<kBehind>(p, prod_sel ? nxt : cur, win, lane);
       }
       // items start on an even page and a window holds 32: both ids are in this window
 #pragma unroll
@@ -901,7 +991,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
   while (cur.valid && !failed) {
     const int hq0 = cur.kvh * p.group + cur.hg * TR::kHeadsPerItem;
     const int nheads = min(TR::kHeadsPerItem, p.group - cur.hg * TR::kHeadsPerItem);
-    const int seq_len = p.seq_lens[cur.seq];
+    const int seq_len = kBehind ? (has_alibi ? __ldcg(p.seq_lens + cur.seq) - pre.prefix_len : 0) : p.seq_lens[cur.seq];
 
     // ---- Q fragments (B operand), head = nt*8 + g
     uint32_t qf[GP][KS][2];
@@ -915,11 +1005,14 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
         uint32_t v0 = 0, v1 = 0;
         if (hl < nheads) {
           if constexpr (!kFp8) {
-            v0 = *reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 2 * c);
-            v1 = *reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 + 2 * c);
+            const uint32_t* q0 = reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 2 * c);
+            const uint32_t* q1 = reinterpret_cast<const uint32_t*>(qrow + 16 * ks + 8 + 2 * c);
+            v0 = kBehind ? __ldcg(q0) : *q0;
+            v1 = kBehind ? __ldcg(q1) : *q1;
           } else {
             // k index 2c+i <-> d 4c+i ; k index 2c+8+i <-> d 4c+2+i ; operands in f16
-            const uint2 raw = *reinterpret_cast<const uint2*>(qrow + 16 * ks + 4 * c);
+            const uint2* q01 = reinterpret_cast<const uint2*>(qrow + 16 * ks + 4 * c);
+            const uint2 raw = kBehind ? __ldcg(q01) : *q01;
             const QT* e = reinterpret_cast<const QT*>(&raw);
             v0 = pack2<false>(to_f32(e[0]), to_f32(e[1]));
             v1 = pack2<false>(to_f32(e[2]), to_f32(e[3]));
@@ -1080,11 +1173,12 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
           tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 8));
           tmax = fmaxf(tmax, __shfl_xor_sync(0xffffffffu, tmax, 16));
           const float m_old = m_run[nt][j];
-          const float m_new = fmaxf(m_old, tmax);
+          float m_new = fmaxf(m_old, tmax);
           // m_new is finite here: every processed page holds at least one valid token
           alpha[nt][j] = fast_exp2(m_old - m_new);
           rescale |= (m_new != m_old);
           m_run[nt][j] = m_new;
+          if (kBehind && m_new == -INFINITY) m_new = alpha[nt][j] = 0.f;  // (logits of -inf: weights of 0, not NaN)
           float psum = 0.f;
 #pragma unroll
           for (int t = 0; t < NT; ++t) {
@@ -1197,6 +1291,64 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
 
     // ---- finalise the item: l over the 8 row groups, normalise, write
     const bool direct = cur.nparts == 1;
+    if constexpr (kBehind) {
+      grid_dependency();  // (the prefix's parts, and the arrival counters)
+#pragma unroll
+      for (int nt = 0; nt < GP; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], o);
+      if (direct) {
+        const SharedPrefixParts::Row r = pre.row<D>(cur.seq, cur.kvh, cur.hg * TR::kHeadsPerItem, p.group);
+        for (int k = 0; k < r.n; ++k) {
+          const unsigned char* part = r.first + k * r.step;
+#pragma unroll
+          for (int nt = 0; nt < GP; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const int hl = nt * 8 + 2 * c + j;
+              if (hl >= nheads) continue;
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + 128 * D * 4) + r.row + hl);
+              const float* val = reinterpret_cast<const float*>(part) + (g >> 2) * 512 + (r.row + hl) * 4 + (g & 3);
+              float v[KS][2];
+#pragma unroll
+              for (int mt = 0; mt < KS; ++mt) {
+                v[mt][0] = __ldcg(val + mt * 2048);
+                v[mt][1] = __ldcg(val + mt * 2048 + 1024);
+              }
+              if (ml.y == 0.f) continue;  // (the row sees no key of this part, which holds no output)
+              const float m_new = fmaxf(m_run[nt][j], ml.x);
+              const float old = m_new == -INFINITY ? 0.f : fast_exp2(m_run[nt][j] - m_new), f = fast_exp2(ml.x - m_new);
+              m_run[nt][j] = m_new;
+              l_run[nt][j] = l_run[nt][j] * old + ml.y * f;
+#pragma unroll
+              for (int mt = 0; mt < KS; ++mt) {
+                o[mt][nt][j] = o[mt][nt][j] * old + v[mt][0] * f;
+                o[mt][nt][2 + j] = o[mt][nt][2 + j] * old + v[mt][1] * f;
+              }
+            }
+        }
+      } else {
+        constexpr int HPI = TR::kHeadsPerItem;
+        const int64_t slot = 2 * int64_t(my_number) + (cur.part == 0);  // (a range ends inside at most two sequences)
+        float* own = reinterpret_cast<float*>(pre.own + slot * (HPI * (D * 4 + 8)));
+#pragma unroll
+        for (int nt = 0; nt < GP; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int hl = nt * 8 + 2 * c + j;
+            if (hl >= nheads) continue;
+            if (g == 0) reinterpret_cast<float2*>(own + HPI * D)[hl] = make_float2(m_run[nt][j], l_run[nt][j]);
+#pragma unroll
+            for (int mt = 0; mt < KS; ++mt) {
+              own[hl * D + 16 * mt + g] = o[mt][nt][j];
+              own[hl * D + 16 * mt + 8 + g] = o[mt][nt][2 + j];
+            }
+          }
+      }
+    }
+    if (!kBehind || direct) {
     QT* obase;
     int64_t ohead_stride;
     if (direct) {
@@ -1213,9 +1365,11 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float l = l_run[nt][j];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
+        if constexpr (!kBehind) {
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+        }
         inv[j] = kv_o * __fdividef(1.f, l + 1e-6f);
         const int hl = nt * 8 + 2 * c + j;
         if (!direct && g == 0 && hl < nheads) {
@@ -1226,7 +1380,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
         }
         if (direct && p.lse != nullptr && g == 0 && hl < nheads)
           p.lse[int64_t(hq0 + hl) * p.num_seqs + cur.seq] =
-              l > 0.f ? (m_run[nt][j] + log2f(l)) * kLn2 : -INFINITY;
+              (kBehind ? l != 0.f : l > 0.f) ? (m_run[nt][j] + log2f(l)) * kLn2 : -INFINITY;
       }
       const int hl_t = nt * 8 + g;  // head owned after the transpose
 #pragma unroll
@@ -1243,6 +1397,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
         }
       }
     }
+    }
 
     // ---- split sequences: the warp that delivers the LAST partial of a (sequence, kv head,
     // head group) merges all of them into `out` (replaces the reference's separate
@@ -1251,7 +1406,27 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
     // and done after the page loop (below), where it costs the loop no registers.  A range has
     // at most two pieces of sequences that continue in other ranges (its first and its last),
     // so two notes per warp are enough.
-    if (!direct && p.arrive != nullptr) {
+    if (kBehind && !direct) {
+      __threadfence();
+      __syncwarp();
+      unsigned old = 0;
+      if (lane == 0)
+        old = atomicAdd(pre.arrive + int64_t(cur.kvh * p.head_groups + cur.hg) * p.num_seqs + cur.seq, 1u);
+      old = __shfl_sync(0xffffffffu, old, 0);
+      if (old == unsigned(cur.nparts - 1)) {
+        const int n = s_ntodo[warp];
+        if (lane == 0) {
+          if (n < 2) {
+            s_todo[warp][n] = make_int4(cur.seq, cur.kvh * p.head_groups + cur.hg, cur.nparts, cur.part);
+            s_ntodo[warp] = n + 1;
+          } else {
+            atomicExch(p.status, kStatusMergeNotes);
+          }
+        }
+        __syncwarp();
+      }
+    }
+    if (!kBehind && !direct && p.arrive != nullptr) {
       __threadfence();  // partials visible before the arrival is counted
       __syncwarp();
       const size_t unit = (size_t(cur.seq) * p.num_kv_heads + cur.kvh) * p.head_groups + cur.hg;
@@ -1320,6 +1495,14 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
       const bool group_first = (td.w >> 30) != 0;
       const int hq0 = kvh * p.group + hg * TR::kHeadsPerItem;
       const int nheads = min(TR::kHeadsPerItem, p.group - hg * TR::kHeadsPerItem);
+      if constexpr (kBehind) {
+        __threadfence();  // order the loads below after the observed arrivals
+        merge_behind<QT, D, TR::kHeadsPerItem>(
+            pre.own + 2 * int64_t(my_number - part) * (TR::kHeadsPerItem * (D * 4 + 8)), nparts, pre,
+            static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + hq0) * D, seq, kvh, hg * TR::kHeadsPerItem, p.group,
+            nheads, lane, kv_o, p.lse ? p.lse + int64_t(hq0) * p.num_seqs + seq : nullptr, p.num_seqs);
+        continue;
+      }
       const size_t unit = (size_t(seq) * p.num_kv_heads + kvh) * p.head_groups + hg;
       const int64_t rowbase = (int64_t(seq) * p.num_heads + hq0) * p.max_partitions;
       QT* tmp_q = static_cast<QT*>(p.tmp_out);
@@ -1365,6 +1548,7 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
     }
   }
 
+  if constexpr (kBehind) return;
   // ---- last CTA out re-arms the scheduler words for the next launch
   __syncthreads();
   if (threadIdx.x == 0) {
@@ -1376,6 +1560,16 @@ __global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodePar
       __threadfence();
     }
   }
+}
+
+template <typename QT, int KV, int D, int GP, int BT, int MAXW>
+__global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_kernel(const DecodeParams p) {
+  decode_persistent<QT, KV, D, GP, BT, MAXW, false>(p, SharedPrefixParts{});
+}
+
+template <typename QT, int KV, int D, int GP, int BT, int MAXW>
+__global__ void __launch_bounds__(MAXW * 32, 1) pa_decode_tails_kernel(const DecodeParams p, const SharedPrefixParts pre) {
+  decode_persistent<QT, KV, D, GP, BT, MAXW, true>(p, pre);
 }
 
 }  // namespace b200pa

@@ -235,19 +235,6 @@ constexpr size_t kSmallRegionBytes = size_t(4) << 20;
 constexpr size_t kWorkspaceBytes = kBigRegionBytes + (kStreamSlots - 1) * kSmallRegionBytes;
 static __device__ __align__(256) unsigned char g_workspace[kWorkspaceBytes];
 
-// Developer knobs, read from the environment once per process (B200PA_TUNE_RELOAD=1 at
-// that first read makes every call read them again, for parameter sweeps in one process).
-struct Tuning {
-  int no_split = 0;      // B200PA_TUNE_NO_SPLIT=1: never use the library workspace
-  int max_parts = 0;     // B200PA_TUNE_MAX_PARTS: cap on partial slots per sequence (>= 2)
-  int min_tokens = 0;    // B200PA_TUNE_MIN_TOKENS: smallest range, in tokens (multiple of 32)
-  int warps = 0;         // B200PA_TUNE_WARPS: warps per CTA
-  int stages = 0;        // B200PA_TUNE_STAGES: ring slots per warp
-  int direct = 0;        // B200PA_TUNE_DIRECT: 1 always the direct kernel where it is built, 2 never
-  int cluster = 0;       // B200PA_TUNE_CLUSTER: its CTAs per cluster
-  int reload = 0;
-};
-
 static int env_int(const char* name, int lo, int hi) {
   const char* e = getenv(name);
   if (e == nullptr || *e == 0) return 0;
@@ -264,11 +251,12 @@ static Tuning read_tuning() {
   t.stages = env_int("B200PA_TUNE_STAGES", 1, 8);
   t.direct = env_int("B200PA_TUNE_DIRECT", 0, 2);
   t.cluster = env_int("B200PA_TUNE_CLUSTER", 1, 16);
+  t.prefix = env_int("B200PA_TUNE_PREFIX", 1, 1024);
   t.reload = env_int("B200PA_TUNE_RELOAD", 0, 1);
   return t;
 }
 
-static Tuning tuning() {
+Tuning tuning() {
   static const Tuning first = read_tuning();
   return first.reload ? read_tuning() : first;
 }

@@ -4,6 +4,7 @@
 
 #include "launch_state.cuh"
 #include "shared_prefix_inst.cuh"
+#include "tails_inst.cuh"
 #include "tensor_map.cuh"
 
 namespace b200pa {
@@ -11,8 +12,51 @@ namespace b200pa {
 struct SharedPrefixPlan {
   SharedPrefixKernels k;  // k.prefix null: the ordinary kernels
   int row_tiles = 0, groups = 0, key_tiles = 0, cut = 0, turns = 0, tiles = 0, grid = 0;
-  int64_t bytes = 0;  // of scratch
+  // behind the prefix: the persistent kernel where tails.fn is not null, else the direct one in clusters
+  TailsKernelInfo tails{nullptr, 0, 1};
+  int warps = 0, slots = 0, min_chunk = 0;
+  size_t smem = 0;
+  int cluster = 1;
+  int64_t items = 0;                            // (sequence, kv head, head group)
+  int64_t own_at = 0, arrive_at = 0, bytes = 0;  // scratch: the prefix's parts, partials, arrivals; its size
 };
+
+static TailsKernelInfo find_tails(int d, int qdt, int kv, int gp, int nt) {
+  switch (d) {
+    case 32: return find_tails_d32(qdt, kv, gp, nt);
+    case 64: return find_tails_d64(qdt, kv, gp, nt);
+    case 80: return find_tails_d80(qdt, kv, gp, nt);
+    case 96: return find_tails_d96(qdt, kv, gp, nt);
+    case 112: return find_tails_d112(qdt, kv, gp, nt);
+    case 128: return find_tails_d128(qdt, kv, gp, nt);
+    case 192: return find_tails_d192(qdt, kv, gp, nt);
+    case 256: return find_tails_d256(qdt, kv, gp, nt);
+  }
+  return {nullptr, 0, 1};
+}
+
+// The persistent kernel's launch, as in attention_entry: two ring slots a warp, as many warps as shared memory and
+// registers have room for (16-bit caches: 12).  False where the table of the sequences does not fit.
+static bool plan_tails(const b200pa_attn_args& a, int gp, SharedPrefixPlan& r) {
+  const int es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1;
+  const TailsKernelInfo ki = find_tails(a.head_size, a.q_dtype, a.kv_dtype, gp, a.block_size / 16);
+  const size_t table = size_t((a.num_seqs + 1 + 3) & ~3) * 4;
+  if (ki.fn == nullptr || table > 48 * 1024) return false;
+  const size_t step = size_t(a.head_size) * a.block_size * es * ki.pages_per_step;
+  const int split = step >= 4096 ? 1 : 0;
+  const size_t slot = split ? step : 2 * step;
+  const size_t budget = 227 * 1024 - 2048 - table - 1024;
+  int w = int(std::min<size_t>(size_t(ki.max_warps), budget / (2 * slot)));
+  if (es == 2 && w > 12) w = 12;
+  if (w >= 8) w &= ~3;
+  if (w < 1) return false;
+  r.tails = ki;
+  r.warps = w;
+  r.slots = 2;
+  r.min_chunk = std::max(2, (64 / a.block_size + 1) & ~1);
+  r.smem = table + ((size_t(w) * r.slots * 8 + 127) & ~size_t(127)) + size_t(w) * r.slots * slot;
+  return true;
+}
 
 static SharedPrefixKernels find_shared_prefix(const b200pa_attn_args& a) {
   const int es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1;
@@ -36,6 +80,7 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   if (a.num_seqs < 2 || prefix_len == 0) return r;
   const SharedPrefixKernels k = find_shared_prefix(a);
   if (k.prefix == nullptr) return r;
+  const Tuning tune = tuning();
   const int sms = sm_count(), group = a.num_heads / a.num_kv_heads, T = 128 / group;
   r.row_tiles = (a.num_seqs + T - 1) / T;
   r.turns = k.row_tiles == 2 && r.row_tiles == 1;
@@ -44,11 +89,30 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   r.tiles = r.turns ? 2 : k.row_tiles;
   r.key_tiles = (prefix_len + k.keys - 1) / k.keys;
   const int64_t items = int64_t(a.num_kv_heads) * r.groups, units = items * r.key_tiles;
-  const int64_t behind = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
-  if (units > INT32_MAX / 2 || behind > INT32_MAX / 16) return r;
-  r.cut = int((units + sms - 1) / sms);
+  if (units > INT32_MAX / 2) return r;
+  const int most = tune.prefix ? std::min(tune.prefix, sms) : sms;
+  r.cut = int((units + most - 1) / most);
   r.grid = int((units + r.cut - 1) / r.cut);
-  r.bytes = (items + r.grid) * r.tiles * int64_t(k.part_bytes);
+  auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
+  r.own_at = up((items + r.grid) * r.tiles * int64_t(k.part_bytes));
+  r.bytes = r.own_at;
+
+  // ---- behind the prefix
+  const int gp = group <= 8 ? 1 : 2, heads = 8 * gp;
+  const int64_t tail_items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + heads - 1) / heads);
+  if (tune.direct != 1 && tail_items <= INT32_MAX / 16 && plan_tails(a, gp, r)) {
+    r.items = tail_items;
+    r.arrive_at = r.own_at + up(2 * int64_t(sms) * r.warps * heads * (a.head_size * 4 + 8));
+    r.bytes = r.arrive_at + up(tail_items * 4);
+  } else {
+    // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
+    r.items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
+    if (r.items > INT32_MAX / 16) return r;
+    const int64_t places = int64_t(sms) * k.ctas_per_sm;
+    const int64_t tiles = (int64_t(std::max(a.max_seq_len - prefix_len, 1)) + 15) / 16;
+    while (r.cluster < 8 && r.items * r.cluster * 10 <= places * 6 && r.cluster * kDirectWarps < tiles) r.cluster *= 2;
+    if (tune.cluster) r.cluster = tune.cluster;
+  }
   r.k = k;
   return r;
 }
@@ -118,6 +182,10 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   p.cut = plan.cut;
   p.turns = plan.turns;
   p.scale = a->scale;
+  if (plan.tails.fn != nullptr) {
+    p.arrive = reinterpret_cast<unsigned*>(p.parts + plan.arrive_at);
+    p.arrivals = int(plan.items);
+  }
   cudaError_t e = plan.k.prefix(p, a->num_heads, plan.grid, s);
   count_launch();
   if (e != cudaSuccess) {
@@ -145,7 +213,6 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   d.max_blocks_per_seq = a->max_num_blocks_per_seq;
   d.len_cap = INT32_MAX;
   d.group = p.group;
-  d.head_groups = (p.group + plan.k.heads - 1) / plan.k.heads;
   d.scale = a->scale;
   d.lse = a->out_lse;
   d.status = p.status;
@@ -158,13 +225,18 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   pre.cut = plan.cut;
   pre.tiles = plan.tiles;
   pre.turns = plan.turns;
-  // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
-  const int64_t items = int64_t(d.num_seqs) * d.num_kv_heads * d.head_groups;
-  const int64_t places = int64_t(sm_count()) * plan.k.ctas_per_sm;
-  const int64_t tiles = (int64_t(std::max(a->max_seq_len - prefix_len, 1)) + 15) / 16;
-  int cluster = 1;
-  while (cluster < 8 && items * cluster * 10 <= places * 6 && cluster * kDirectWarps < tiles) cluster *= 2;
-  e = plan.k.behind(d, pre, int(items), cluster, s);
+  if (plan.tails.fn != nullptr) {
+    d.head_groups = (p.group + (p.group <= 8 ? 8 : 16) - 1) / (p.group <= 8 ? 8 : 16);
+    d.nstages = plan.slots;
+    d.use_table = 1;
+    d.min_chunk = plan.min_chunk;
+    pre.own = p.parts + plan.own_at;
+    pre.arrive = p.arrive;
+    e = plan.tails.fn(d, pre, sm_count(), plan.warps * 32, plan.smem, s);
+  } else {
+    d.head_groups = (p.group + plan.k.heads - 1) / plan.k.heads;
+    e = plan.k.behind(d, pre, int(plan.items), plan.cluster, s);
+  }
   count_launch();
   if (e != cudaSuccess) {
     set_error("shared prefix decode kernel launch failed: %s", cudaGetErrorString(e));

@@ -9,8 +9,8 @@
 //     with as many rows as there are (sequence, query head of a kv head) pairs: tcgen05 tiles of 128 rows x 128 keys,
 //     the pipeline of the prefill kernel (prefill_kernel.cuh: operand layouts, softmax in two halves, roles of the
 //     warps), without a causal edge and without a plan on the device: all items cost the same.
-//   * the direct decode kernel (decode_direct.cuh) takes every sequence's own tokens, adds the prefix's part to its
-//     accumulators, in fp32, and writes the result.
+//   * a decode kernel (decode_kernel.cuh, or decode_direct.cuh where there is little of them) takes every sequence's own
+//     tokens, adds the prefix's part to its accumulators, in fp32, and writes the result.
 // The work of this kernel is a flat list (kv head, group of row tiles, key tile), cut into equal ranges, one to a CTA;
 // a range may cover the end of one item and the start of the next.  What a CTA has of an item goes to a slot of the
 // scratch: item + CTA is a number of its own for every such pair, so nothing is counted and nobody waits.
@@ -31,7 +31,9 @@ struct SharedPrefixParams {
   const int* seq_lens;
   const float* alibi;
   const float* k_scale;
-  unsigned char* parts;       // slots of shared_prefix_slot_bytes(D) * tiles per slot
+  unsigned char* parts;       // slots of one or two row tiles' parts
+  unsigned* arrive;           // counters of the launch behind, to be zeroed
+  int arrivals;
   int* status;
   int64_t q_stride;
   int64_t kv_block_stride;    // elements
@@ -119,6 +121,7 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
   const uint32_t tmem = s_tmem;
   // (the launch behind this one may start now: it waits for this grid before it reads a part)
   grid_dependency();
+  for (int i = blockIdx.x * kPrefillThreads + tid; i < p.arrivals; i += gridDim.x * kPrefillThreads) p.arrive[i] = 0;
 
   const int G = p.group, B = p.block_size, b_shift = 31 - __clz(B);
   const int T = 128 / G;  // sequences of a row tile

@@ -1,0 +1,8 @@
+// The persistent decode kernel behind a shared prefix for head size 64.
+#include "tails_inst.cuh"
+
+namespace b200pa {
+TailsKernelInfo find_tails_d64(int q_dtype, int kv_dtype, int gp, int nt) {
+  return find_tails_for<64>(q_dtype, kv_dtype, gp, nt);
+}
+}  // namespace b200pa
