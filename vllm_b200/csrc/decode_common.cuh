@@ -58,6 +58,33 @@ struct DecodeParams {
   int early;  // 1: the launch in front is the step's KV write, see launch_dependent
 };
 
+// How the SMs are divided between the prefix and what is behind it, where both run at once: by
+// what either takes, ns, from the real lengths.  Integers, so that both kernels come to the same.
+struct SharedPrefixBalance {
+  int64_t prefix;        // of one SM, in all
+  int64_t block;         // of one SM, per cache block of one item behind the prefix
+  int64_t block_hbm;     // of all SMs, in thousandths: what HBM takes at least
+  int64_t prefix_start;  // before and behind the work itself
+  int64_t behind_start;
+  int sms;
+  // CTAs for the prefix, when `blocks` cache blocks are behind it
+  __device__ __forceinline__ int prefix_ctas(int64_t blocks) const {
+    int lo = 1, hi = sms - 1;  // the fewest with which the prefix is not last
+    while (lo < hi) {
+      const int g = (lo + hi) >> 1;
+      const int64_t tp = prefix_start + prefix / g;
+      const int64_t tb = behind_start + max(blocks * block / (sms - g), blocks * block_hbm / 1000);
+      if (tp <= tb) hi = g; else lo = g + 1;
+    }
+    return lo;
+  }
+};
+
+// Cache blocks that a sequence of `len` tokens counts for: an even number, of two at least.
+__device__ __forceinline__ int work_units(int len, int block_size) {
+  return max(2, ((len + block_size - 1) / block_size + 1) & ~1);
+}
+
 // What the launch in front has of a prefix that all sequences share (shared_prefix_kernel.cuh): which part of
 // it covers what, for the kernels that have the sequences' own tokens and add the prefix to them.
 struct SharedPrefixParts {
@@ -69,10 +96,10 @@ struct SharedPrefixParts {
   int cut;        // key tiles of a CTA
   int tiles;      // row tiles of a group that a slot holds: 2, or 1
   int turns;      // 1: a slot's two tiles are parts of the same rows
-  // the persistent kernel's own: partials of sequences that are cut (two slots to a range), arrivals at every item
-  // (zeroed by the prefix's kernel)
+  // where the persistent kernel is behind: its partials (slot item + range), and every item's first range and partials
   unsigned char* own;
-  unsigned* arrive;
+  int2* found;
+  SharedPrefixBalance balance;
 
   // The parts of a row (`head`: of its kv head's group) at head size D: the first, bytes between two, how many;
   // its place in them.  They lie in slots item + CTA, of the CTAs whose ranges meet the row's item.

@@ -90,8 +90,9 @@ struct DirectShape {
 };
 
 // grid.x = (sequence, kv head, head group) items x cluster size.  kBehind: attends to what a sequence has behind the
-// shared prefix, and adds the prefix's parts.
-template <typename QT, int KV, int D, int GP, bool kBehind>
+// shared prefix, and adds the prefix's parts.  kSolo (many short sequences): every warp has an item of its own, nothing
+// is merged between warps; `cluster` is the number of items then.
+template <typename QT, int KV, int D, int GP, bool kBehind, bool kSolo = false>
 __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int cluster, const SharedPrefixParts& pre) {
   using TR = DecodeTraits<QT, KV, D, GP>;
   using SH = DirectShape<KV, D, GP>;
@@ -113,8 +114,9 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, c = lane & 3;
-  const int rank = cluster == 1 ? 0 : int(cluster_rank());
-  int item = int(blockIdx.x) / cluster;
+  const int rank = kSolo || cluster == 1 ? 0 : int(cluster_rank());
+  int item = kSolo ? int(blockIdx.x) * kDirectWarps + warp : int(blockIdx.x) / cluster;
+  if (kSolo && item >= cluster) return;
   const int hg = item % p.head_groups;
   item /= p.head_groups;
   const int kvh = item % p.num_kv_heads;
@@ -169,7 +171,7 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
 
   // ---- this warp's 16-token tiles [t_begin, t_end)
   const int tiles = (len + 15) >> 4;
-  const int nw = cluster * kDirectWarps, gw = rank * kDirectWarps + warp;
+  const int nw = kSolo ? 1 : cluster * kDirectWarps, gw = kSolo ? 0 : rank * kDirectWarps + warp;
   const int t_begin = int(int64_t(tiles) * gw / nw), t_end = int(int64_t(tiles) * (gw + 1) / nw);
   const int* bt = p.block_tables + int64_t(seq) * p.max_blocks_per_seq;
   const char* kb = static_cast<const char*>(p.kc) + int64_t(kvh) * p.kv_head_stride * ES;
@@ -372,6 +374,58 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
         }
       }
     }
+  if constexpr (kSolo) {
+    // a lane has one head, and every (32 / heads)th group of four dimensions of it
+    __syncwarp();
+    grid_dependency();  // (from here on the prefix's parts)
+    const int heads = nheads <= 1 ? 1 : 1 << (32 - __clz(nheads - 1));
+    const int hl = lane & (heads - 1), d_first = lane / heads, d_step = 32 / heads;
+    const bool on = hl < nheads;
+    const SharedPrefixParts::Row r = pre.row<D>(seq, kvh, hg * HEADS + (on ? hl : 0), p.group);
+    const float scale = kFp8 ? __ldcg(p.v_scale) : 1.f;
+    constexpr int NU = 8;  // groups at a time
+    for (int d0 = d_first; d0 < D / 4; d0 += NU * d_step) {
+      float2 st = s_ml[warp][on ? hl : 0];
+      float m = st.x, l = on ? st.y : 0.f;
+      float4 acc[NU];
+#pragma unroll
+      for (int i = 0; i < NU; ++i)
+        acc[i] = l != 0.f && d0 + i * d_step < D / 4
+                     ? *reinterpret_cast<const float4*>(mine + hl * ROW + (d0 + i * d_step) * 4)
+                     : make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < r.n; ++k) {
+        const unsigned char* q = r.first + k * r.step;
+        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + 128 * D * 4) + r.row);
+        float4 v[NU];
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+          v[i] = __ldcg(reinterpret_cast<const float4*>(q) + min(d0 + i * d_step, D / 4 - 1) * 128 + r.row);
+        if (ml.y == 0.f) continue;  // (a part in which the row has no key holds no output)
+        const float m_new = fmaxf(m, ml.x);
+        const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new), f = fast_exp2(ml.x - m_new);
+        m = m_new;
+        l = l * old + ml.y * f;
+#pragma unroll
+        for (int i = 0; i < NU; ++i)
+          acc[i] = make_float4(acc[i].x * old + v[i].x * f, acc[i].y * old + v[i].y * f, acc[i].z * old + v[i].z * f,
+                               acc[i].w * old + v[i].w * f);
+      }
+      if (!on) continue;
+      const float inv = scale * __fdividef(1.f, l + 1e-6f);
+#pragma unroll
+      for (int i = 0; i < NU; ++i) {
+        const int d = (d0 + i * d_step) * 4;
+        if (d >= D) break;
+        uint2 w;
+        w.x = pack2<kOutBf>(acc[i].x * inv, acc[i].y * inv);
+        w.y = pack2<kOutBf>(acc[i].z * inv, acc[i].w * inv);
+        *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + hq0 + hl) * D + d) = w;
+      }
+      if (p.lse != nullptr && d0 == 0)
+        p.lse[int64_t(hq0 + hl) * p.num_seqs + seq] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    }
+    return;
+  }
   __syncthreads();
 
   // ---- merges.  A unit is four head dimensions of one head.
@@ -509,6 +563,12 @@ template <typename QT, int KV, int D, int GP>
 __global__ void __launch_bounds__(kDirectWarps * 32, DirectShape<KV, D, GP>::kMinCtas)
 pa_decode_behind_kernel(const DecodeParams p, const SharedPrefixParts pre, const int cluster) {
   decode_direct<QT, KV, D, GP, true>(p, cluster, pre);
+}
+
+template <typename QT, int KV, int D, int GP>
+__global__ void __launch_bounds__(kDirectWarps * 32, DirectShape<KV, D, GP>::kMinCtas)
+pa_decode_solo_kernel(const DecodeParams p, const SharedPrefixParts pre, const int items) {
+  decode_direct<QT, KV, D, GP, true, true>(p, items, pre);
 }
 
 }  // namespace b200pa

@@ -91,7 +91,6 @@ __device__ __forceinline__ int load_bt(const DecodeParams& p, const WorkItem& it
 // partial (kept in the group's first slot), and the warp that completes the last group merges
 // the groups.  One warp merging 60 partials of four heads takes ~14 us, which would be the
 // tail of the launch; groups are merged by different warps as they finish.
-constexpr int kBehindPieces = 32;  // that a sequence is cut into at most, behind a shared prefix
 constexpr int kMergeFan = 8;
 constexpr int kMergeDirectMax = 32;  // (16 measured 2 % slower on a 4-way kv-head shard, equal elsewhere)
 
@@ -523,89 +522,9 @@ __device__ __forceinline__ void merge_partials(float* exp_sums, float* max_logit
   }
 }
 
-// The merge of a sequence that was cut, behind a shared prefix: `np` partials of `nheads` heads and the prefix's parts.
-// (Partials: the first in slot 1 of its range, the others in slot 0 of the ranges behind it, two slots to a range.)  A lane owns four head dimensions (of each 128), four heads at a time; of every source, two at a time,
-// statistics and output are requested together.
-template <typename QT, int D, int HEADS>
-__device__ __noinline__ void merge_behind(const unsigned char* own, int np, const SharedPrefixParts& pre, QT* out,
-                                          int seq, int kvh, int head0, int group, int nheads, int lane, float scale,
-                                          float* lse, int lse_stride) {
-  constexpr bool kOutBf = std::is_same_v<QT, __nv_bfloat16>;
-  constexpr int kSlot = HEADS * (D * 4 + 8);
-  const SharedPrefixParts::Row r = pre.row<D>(seq, kvh, head0, group);
-  const int n = np + r.n;
-  for (int h0 = 0; h0 < nheads; h0 += 4) {
-    const int nh = min(4, nheads - h0);
-    for (int d = lane * 4; d < (D + 127) / 128 * 128; d += 128) {
-      const bool in = d < D;
-      const int dd = in ? d : 0;
-      float4 acc[4];
-      float m[4], l[4];
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        acc[h] = make_float4(0.f, 0.f, 0.f, 0.f);
-        m[h] = -INFINITY;
-        l[h] = 0.f;
-      }
-      for (int k0 = 0; k0 < n; k0 += 2) {
-        float2 ml[2][4];
-        float4 v[2][4];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const int s = min(k0 + k, n - 1);
-          const unsigned char* q = s < np ? own + (2 * int64_t(s) + (s == 0)) * kSlot : r.first + (s - np) * r.step;
-          const unsigned char* stat = s < np ? q + HEADS * D * 4 + h0 * 8 : q + 128 * D * 4 + (r.row + h0) * 8;
-          const unsigned char* val = s < np ? q + (h0 * D + dd) * 4 : q + (dd * 32 + r.row + h0) * 16;
-          const int step = s < np ? D * 4 : 16;
-#pragma unroll
-          for (int h = 0; h < 4; ++h) {
-            const int hh = h < nh ? h : 0;
-            ml[k][h] = __ldcg(reinterpret_cast<const float2*>(stat + hh * 8));
-            v[k][h] = __ldcg(reinterpret_cast<const float4*>(val + hh * step));
-            if (k0 + k >= n) ml[k][h] = make_float2(-INFINITY, 0.f);
-          }
-        }
-#pragma unroll
-        for (int h = 0; h < 4; ++h) {
-          float m_new = m[h];
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (ml[k][h].y != 0.f) m_new = fmaxf(m_new, ml[k][h].x);
-          const float old = m_new == -INFINITY ? 0.f : fast_exp2(m[h] - m_new);
-          l[h] *= old;
-          acc[h] = make_float4(acc[h].x * old, acc[h].y * old, acc[h].z * old, acc[h].w * old);
-          m[h] = m_new;
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (ml[k][h].y != 0.f) {  // (what has no key has written no output)
-              const float f = fast_exp2(ml[k][h].x - m_new);
-              l[h] += ml[k][h].y * f;
-              acc[h].x += f * v[k][h].x;
-              acc[h].y += f * v[k][h].y;
-              acc[h].z += f * v[k][h].z;
-              acc[h].w += f * v[k][h].w;
-            }
-          }
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < 4; ++h) {
-        if (h >= nh) break;
-        const float inv = scale * __fdividef(1.f, l[h] + 1e-6f);
-        if (in) {
-          uint2 w;
-          w.x = pack2<kOutBf>(acc[h].x * inv, acc[h].y * inv);
-          w.y = pack2<kOutBf>(acc[h].z * inv, acc[h].w * inv);
-          *reinterpret_cast<uint2*>(out + (h0 + h) * D + d) = w;
-        }
-        if (lse != nullptr && d == 0) lse[int64_t(h0 + h) * lse_stride] = l[h] != 0.f ? (m[h] + log2f(l[h])) * kLn2 : -INFINITY;
-      }
-    }
-  }
-}
-
-// kBehind: attends to what the sequences have behind a shared prefix and adds the prefix's parts (split launches only;
-// partials and arrival counters are in the scratch of the call, partials in fp32).
+// kBehind: attends to what the sequences have behind a shared prefix, on the SMs that the prefix's kernel, which runs
+// beside it, leaves.  Split launches only; every piece of a sequence leaves an fp32 partial in the scratch of the call,
+// which a third kernel adds to the prefix's (shared_prefix_kernel.cuh).
 template <typename QT, int KV, int D, int GP, int BT, int MAXW, bool kBehind>
 __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const SharedPrefixParts& pre) {
   using TR = DecodeTraits<QT, KV, D, GP>;
@@ -654,8 +573,8 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
   __shared__ int4 s_iter[MAXW];  // per warp: units left, block offset, sequence, head
   __shared__ int4 s_todo[MAXW][2];  // per warp: merges owed (sequence, head item, pieces, piece | level)
   __shared__ int s_ntodo[MAXW];
-  // (kBehind: the prefix's kernel lets this one in when all before it is complete; what is read up to the wait for its
-  // parts is read past L1, and by copies of another proxy behind a fence)
+  // (kBehind: the prefix's kernel lets this one in when all before it is complete, and writes nothing that is read here.
+  // What is read without a wait of this grid is read past L1, and by copies of another proxy behind a fence)
   if (!kBehind && !p.early) grid_dependency();
   if (kBehind && lane == 0) asm volatile("fence.proxy.async.global;" ::: "memory");
   const bool flat = kBehind || p.use_table != 0;
@@ -669,7 +588,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     const int s1 = min(S, s0 + per);
     auto units_of = [&](int s) {
       const int len = kBehind ? max(__ldcg(p.seq_lens + s) - pre.prefix_len, 0) : min(max(__ldcg(p.seq_lens + s), 0), p.len_cap);
-      return max(2, ((len + B - 1) / B + 1) & ~1);
+      return work_units(len, B);
     };
     int mine = 0, mx = 0;
     for (int s = s0; s < s1; ++s) {
@@ -708,11 +627,12 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
       // pieces than the scratch has slots per sequence (a sequence of n units meets at most
       // (n - 1) / C + 2 ranges).  Even, see above.
       const long long U = (long long)hsubs * total;
-      const long long W = (long long)gridDim.x * nwarps;
+      const int ctas = kBehind ? pre.balance.sms - pre.balance.prefix_ctas(U) : int(gridDim.x);
+      if (kBehind) s_plan[3] = ctas;
+      const long long W = (long long)ctas * nwarps;
       long long C = (U + W - 1) / W;
       C = max(C, (long long)p.min_chunk);
-      // (kBehind: any number of slots, but one warp merges them)
-      C = max(C, (long long)((n_max - 1) / (kBehind ? kBehindPieces - 1 : max(1, p.max_partitions - 1)) + 1));
+      if (!kBehind) C = max(C, (long long)((n_max - 1) / max(1, p.max_partitions - 1) + 1));
       C = (C + 1) & ~1ll;
       s_plan[0] = int(min(C, (long long)INT32_MAX - 1));
       s_plan[1] = total;
@@ -727,13 +647,18 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     for (int s = threadIdx.x; s < p.num_seqs; s += blockDim.x) prefetch_l1(p.seq_lens + s);
   __syncthreads();
 
-  const unsigned grid_warps = gridDim.x * unsigned(nwarps);
+  const unsigned ctas = kBehind ? unsigned(s_plan[3]) : gridDim.x;
+  if (kBehind && blockIdx.x >= ctas) {
+    grid_dependency();
+    return;
+  }
+  const unsigned grid_warps = ctas * unsigned(nwarps);
   // work items of an unsplit launch / ranges of a split one
   const unsigned total_items = flat ? unsigned(s_plan[2]) : unsigned(p.num_seqs) * unsigned(hsubs);
   // Ranges and the first items are numbered SM-first: warp w of CTA b has number
   // w * gridDim.x + b, so a launch with fewer of them than warps leaves the
   // highest-numbered warps of every CTA idle.
-  const unsigned my_number = unsigned(warp) * gridDim.x + blockIdx.x;
+  const unsigned my_number = unsigned(warp) * ctas + blockIdx.x;
 
   // Ring of this warp.  The host sizes warps and slots without knowing the lengths; when the
   // batch turns out to have fewer ranges / items than the grid has warps, the warps without
@@ -741,7 +666,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
   // in flight, which is what a launch bound by the latency of one item needs.
   int NSLOT = slots_per_warp;
   if (total_items < grid_warps) {
-    const int busy = max(1, int((total_items + gridDim.x - 1) / gridDim.x));  // per CTA, at most
+    const int busy = max(1, int((total_items + ctas - 1) / ctas));  // per CTA, at most
     NSLOT = min(8, nwarps * slots_per_warp / busy);
   }
   const uint32_t my_slot0 = smem_u32(slots) + uint32_t(warp) * NSLOT * slot_bytes;
@@ -1219,6 +1144,27 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
         const int r = rem - pl * B;               // valid tokens in that block
         unsigned char* vpage = my_slots + size_t(cons_slot) * slot_bytes +
                                (split_kv ? 0u : step_bytes) + pl * page_bytes;
+        if constexpr (kBehind) {
+          // the 16 tokens of the last tile that is multiplied, 16 bytes at a time.  (Short sequences are masked
+          // often: 2000 of 8 to 250 tokens, 64 / 8 heads, fp8, 185 us with the loop below.)
+          const int left = r & 15;  // valid tokens of the tile (0: all)
+          if (left != 0) {
+            for (int d = lane; d < D; d += 32) {
+              uint4* row = reinterpret_cast<uint4*>(vpage + (d * B + (r & ~15)) * ES);
+#pragma unroll
+              for (int q = 0; q < ES; ++q) {
+                const int bits = min(max((left * ES - 16 * q) * 8, 0), 128);  // of these 16 bytes that stay
+                if (bits == 128) continue;
+                uint4 v = row[q];
+                auto keep = [&](uint32_t w, int at) {
+                  const int n = bits - at;
+                  return n >= 32 ? w : n <= 0 ? 0u : w & (0xffffffffu >> (32 - n));
+                };
+                row[q] = make_uint4(keep(v.x, 0), keep(v.y, 32), keep(v.z, 64), keep(v.w, 96));
+              }
+            }
+          }
+        } else
         for (int d = lane; d < D; d += 32) {
           for (int tk = r; tk < B; ++tk) {
             if constexpr (ES == 1) vpage[d * B + tk] = 0;
@@ -1292,63 +1238,30 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     // ---- finalise the item: l over the 8 row groups, normalise, write
     const bool direct = cur.nparts == 1;
     if constexpr (kBehind) {
-      grid_dependency();  // (the prefix's parts, and the arrival counters)
+      // the piece's part, as the prefix's: O as [4 dimensions][heads] in fp32, then (m, l) of the heads
+      constexpr int HPI = TR::kHeadsPerItem;
+      const int64_t item = int64_t(cur.kvh * p.head_groups + cur.hg) * p.num_seqs + cur.seq;
+      if (cur.part == 0 && lane == 0) pre.found[item] = make_int2(int(my_number), cur.nparts);
+      float* own = reinterpret_cast<float*>(pre.own + (item + my_number) * (HPI * (D * 4 + 8)));
 #pragma unroll
       for (int nt = 0; nt < GP; ++nt)
 #pragma unroll
-        for (int j = 0; j < 2; ++j)
+        for (int j = 0; j < 2; ++j) {
+          float l = l_run[nt][j];
+          l += __shfl_xor_sync(0xffffffffu, l, 4);
+          l += __shfl_xor_sync(0xffffffffu, l, 8);
+          l += __shfl_xor_sync(0xffffffffu, l, 16);
+          const int hl = nt * 8 + 2 * c + j;
+          if (hl >= nheads) continue;
+          if (g == 0) reinterpret_cast<float2*>(own + HPI * D)[hl] = make_float2(m_run[nt][j], l);
 #pragma unroll
-          for (int o = 4; o < 32; o <<= 1) l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], o);
-      if (direct) {
-        const SharedPrefixParts::Row r = pre.row<D>(cur.seq, cur.kvh, cur.hg * TR::kHeadsPerItem, p.group);
-        for (int k = 0; k < r.n; ++k) {
-          const unsigned char* part = r.first + k * r.step;
-#pragma unroll
-          for (int nt = 0; nt < GP; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              const int hl = nt * 8 + 2 * c + j;
-              if (hl >= nheads) continue;
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(part + 128 * D * 4) + r.row + hl);
-              const float* val = reinterpret_cast<const float*>(part) + (g >> 2) * 512 + (r.row + hl) * 4 + (g & 3);
-              float v[KS][2];
-#pragma unroll
-              for (int mt = 0; mt < KS; ++mt) {
-                v[mt][0] = __ldcg(val + mt * 2048);
-                v[mt][1] = __ldcg(val + mt * 2048 + 1024);
-              }
-              if (ml.y == 0.f) continue;  // (the row sees no key of this part, which holds no output)
-              const float m_new = fmaxf(m_run[nt][j], ml.x);
-              const float old = m_new == -INFINITY ? 0.f : fast_exp2(m_run[nt][j] - m_new), f = fast_exp2(ml.x - m_new);
-              m_run[nt][j] = m_new;
-              l_run[nt][j] = l_run[nt][j] * old + ml.y * f;
-#pragma unroll
-              for (int mt = 0; mt < KS; ++mt) {
-                o[mt][nt][j] = o[mt][nt][j] * old + v[mt][0] * f;
-                o[mt][nt][2 + j] = o[mt][nt][2 + j] * old + v[mt][1] * f;
-              }
-            }
-        }
-      } else {
-        constexpr int HPI = TR::kHeadsPerItem;
-        const int64_t slot = 2 * int64_t(my_number) + (cur.part == 0);  // (a range ends inside at most two sequences)
-        float* own = reinterpret_cast<float*>(pre.own + slot * (HPI * (D * 4 + 8)));
-#pragma unroll
-        for (int nt = 0; nt < GP; ++nt)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int hl = nt * 8 + 2 * c + j;
-            if (hl >= nheads) continue;
-            if (g == 0) reinterpret_cast<float2*>(own + HPI * D)[hl] = make_float2(m_run[nt][j], l_run[nt][j]);
-#pragma unroll
-            for (int mt = 0; mt < KS; ++mt) {
-              own[hl * D + 16 * mt + g] = o[mt][nt][j];
-              own[hl * D + 16 * mt + 8 + g] = o[mt][nt][2 + j];
-            }
+          for (int mt = 0; mt < KS; ++mt) {
+            float* at = own + ((4 * mt + (g >> 2)) * HPI + hl) * 4 + (g & 3);
+            at[0] = o[mt][nt][j];
+            at[2 * HPI * 4] = o[mt][nt][2 + j];
           }
-      }
-    }
-    if (!kBehind || direct) {
+        }
+    } else {
     QT* obase;
     int64_t ohead_stride;
     if (direct) {
@@ -1365,11 +1278,9 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float l = l_run[nt][j];
-        if constexpr (!kBehind) {
-          l += __shfl_xor_sync(0xffffffffu, l, 4);
-          l += __shfl_xor_sync(0xffffffffu, l, 8);
-          l += __shfl_xor_sync(0xffffffffu, l, 16);
-        }
+        l += __shfl_xor_sync(0xffffffffu, l, 4);
+        l += __shfl_xor_sync(0xffffffffu, l, 8);
+        l += __shfl_xor_sync(0xffffffffu, l, 16);
         inv[j] = kv_o * __fdividef(1.f, l + 1e-6f);
         const int hl = nt * 8 + 2 * c + j;
         if (!direct && g == 0 && hl < nheads) {
@@ -1380,7 +1291,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
         }
         if (direct && p.lse != nullptr && g == 0 && hl < nheads)
           p.lse[int64_t(hq0 + hl) * p.num_seqs + cur.seq] =
-              (kBehind ? l != 0.f : l > 0.f) ? (m_run[nt][j] + log2f(l)) * kLn2 : -INFINITY;
+              l > 0.f ? (m_run[nt][j] + log2f(l)) * kLn2 : -INFINITY;
       }
       const int hl_t = nt * 8 + g;  // head owned after the transpose
 #pragma unroll
@@ -1406,26 +1317,6 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     // and done after the page loop (below), where it costs the loop no registers.  A range has
     // at most two pieces of sequences that continue in other ranges (its first and its last),
     // so two notes per warp are enough.
-    if (kBehind && !direct) {
-      __threadfence();
-      __syncwarp();
-      unsigned old = 0;
-      if (lane == 0)
-        old = atomicAdd(pre.arrive + int64_t(cur.kvh * p.head_groups + cur.hg) * p.num_seqs + cur.seq, 1u);
-      old = __shfl_sync(0xffffffffu, old, 0);
-      if (old == unsigned(cur.nparts - 1)) {
-        const int n = s_ntodo[warp];
-        if (lane == 0) {
-          if (n < 2) {
-            s_todo[warp][n] = make_int4(cur.seq, cur.kvh * p.head_groups + cur.hg, cur.nparts, cur.part);
-            s_ntodo[warp] = n + 1;
-          } else {
-            atomicExch(p.status, kStatusMergeNotes);
-          }
-        }
-        __syncwarp();
-      }
-    }
     if (!kBehind && !direct && p.arrive != nullptr) {
       __threadfence();  // partials visible before the arrival is counted
       __syncwarp();
@@ -1480,13 +1371,22 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
       nxt = decode(nn_raw);
       nn_raw = fetch();
     }
+    if constexpr (kBehind) {  // the next item's queries are on their way when it becomes the current one
+      if (nxt.valid) {
+        const int bytes = min(TR::kHeadsPerItem, p.group - nxt.hg * TR::kHeadsPerItem) * D * 2;
+        const char* q = reinterpret_cast<const char*>(
+            static_cast<const QT*>(p.q) + int64_t(nxt.seq) * p.q_stride +
+            int64_t(nxt.kvh * p.group + nxt.hg * TR::kHeadsPerItem) * D);
+        for (int i = lane * 128; i < bytes; i += 32 * 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(q + i));
+      }
+    }
     // the producer either already works on the new `cur` (keep its state) or starts it now
     if (prod_sel == 1) prod_sel = 0; else producer_take(cur);
     while (inflight < NSLOT && produce_one()) {}
   }
 
   // ---- the merges this warp owes (noted above)
-  if (!failed) {
+  if (!kBehind && !failed) {
     const int ntodo = s_ntodo[warp];
     for (int k = 0; k < ntodo; ++k) {
       const int4 td = s_todo[warp][k];
@@ -1495,14 +1395,6 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
       const bool group_first = (td.w >> 30) != 0;
       const int hq0 = kvh * p.group + hg * TR::kHeadsPerItem;
       const int nheads = min(TR::kHeadsPerItem, p.group - hg * TR::kHeadsPerItem);
-      if constexpr (kBehind) {
-        __threadfence();  // order the loads below after the observed arrivals
-        merge_behind<QT, D, TR::kHeadsPerItem>(
-            pre.own + 2 * int64_t(my_number - part) * (TR::kHeadsPerItem * (D * 4 + 8)), nparts, pre,
-            static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + hq0) * D, seq, kvh, hg * TR::kHeadsPerItem, p.group,
-            nheads, lane, kv_o, p.lse ? p.lse + int64_t(hq0) * p.num_seqs + seq : nullptr, p.num_seqs);
-        continue;
-      }
       const size_t unit = (size_t(seq) * p.num_kv_heads + kvh) * p.head_groups + hg;
       const int64_t rowbase = (int64_t(seq) * p.num_heads + hq0) * p.max_partitions;
       QT* tmp_q = static_cast<QT*>(p.tmp_out);
@@ -1548,7 +1440,10 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     }
   }
 
-  if constexpr (kBehind) return;
+  if constexpr (kBehind) {
+    grid_dependency();  // (so that this grid's end is the prefix's as well)
+    return;
+  }
   // ---- last CTA out re-arms the scheduler words for the next launch
   __syncthreads();
   if (threadIdx.x == 0) {

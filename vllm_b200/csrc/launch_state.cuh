@@ -34,6 +34,7 @@ struct Tuning {
   int stages = 0;        // B200PA_TUNE_STAGES: ring slots per warp
   int direct = 0;        // B200PA_TUNE_DIRECT: 1 always the direct kernel where it is built, 2 never
   int cluster = 0;       // B200PA_TUNE_CLUSTER: its CTAs per cluster
+  int behind = 0;        // B200PA_TUNE_BEHIND: 1 direct, 2 solo, 3 persistent kernel behind a shared prefix
   int prefix = 0;        // B200PA_TUNE_PREFIX: most CTAs of a shared prefix's kernel
   int reload = 0;
 };

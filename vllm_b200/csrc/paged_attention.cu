@@ -251,6 +251,7 @@ static Tuning read_tuning() {
   t.stages = env_int("B200PA_TUNE_STAGES", 1, 8);
   t.direct = env_int("B200PA_TUNE_DIRECT", 0, 2);
   t.cluster = env_int("B200PA_TUNE_CLUSTER", 1, 16);
+  t.behind = env_int("B200PA_TUNE_BEHIND", 1, 3);
   t.prefix = env_int("B200PA_TUNE_PREFIX", 1, 1024);
   t.reload = env_int("B200PA_TUNE_RELOAD", 0, 1);
   return t;

@@ -12,13 +12,15 @@ namespace b200pa {
 struct SharedPrefixPlan {
   SharedPrefixKernels k;  // k.prefix null: the ordinary kernels
   int row_tiles = 0, groups = 0, key_tiles = 0, cut = 0, turns = 0, tiles = 0, grid = 0;
-  // behind the prefix: the persistent kernel where tails.fn is not null, else the direct one in clusters
+  // behind the prefix: the persistent kernel beside it and a third that adds up, where tails.fn is not null; else the
+  // direct one in clusters, or a warp to an item
   TailsKernelInfo tails{nullptr, 0, 1};
   int warps = 0, slots = 0, min_chunk = 0;
   size_t smem = 0;
-  int cluster = 1;
+  int cluster = 1;  // 0: every warp an item of its own
   int64_t items = 0;                            // (sequence, kv head, head group)
-  int64_t own_at = 0, arrive_at = 0, bytes = 0;  // scratch: the prefix's parts, partials, arrivals; its size
+  SharedPrefixBalance balance{};
+  int64_t own_at = 0, found_at = 0, bytes = 0;  // scratch: the prefix's parts, partials, their places; its size
 };
 
 static TailsKernelInfo find_tails(int d, int qdt, int kv, int gp, int nt) {
@@ -50,9 +52,12 @@ static bool plan_tails(const b200pa_attn_args& a, int gp, SharedPrefixPlan& r) {
   if (es == 2 && w > 12) w = 12;
   if (w >= 8) w &= ~3;
   if (w < 1) return false;
+  r.slots = 2;
+  const Tuning tune = tuning();
+  if (tune.warps) w = std::min(w, tune.warps);
+  if (tune.stages) r.slots = std::max(split ? 2 : 1, std::min(int(budget / (size_t(w) * slot)), tune.stages));
   r.tails = ki;
   r.warps = w;
-  r.slots = 2;
   r.min_chunk = std::max(2, (64 / a.block_size + 1) & ~1);
   r.smem = table + ((size_t(w) * r.slots * 8 + 127) & ~size_t(127)) + size_t(w) * r.slots * slot;
   return true;
@@ -90,9 +95,9 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   r.key_tiles = (prefix_len + k.keys - 1) / k.keys;
   const int64_t items = int64_t(a.num_kv_heads) * r.groups, units = items * r.key_tiles;
   if (units > INT32_MAX / 2) return r;
-  const int most = tune.prefix ? std::min(tune.prefix, sms) : sms;
-  r.cut = int((units + most - 1) / most);
+  r.cut = int((units + sms - 1) / sms);
   r.grid = int((units + r.cut - 1) / r.cut);
+  const int es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1;
   auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
   r.own_at = up((items + r.grid) * r.tiles * int64_t(k.part_bytes));
   r.bytes = r.own_at;
@@ -100,10 +105,21 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   // ---- behind the prefix
   const int gp = group <= 8 ? 1 : 2, heads = 8 * gp;
   const int64_t tail_items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + heads - 1) / heads);
-  if (tune.direct != 1 && tail_items <= INT32_MAX / 16 && plan_tails(a, gp, r)) {
+  if (tune.behind == 3 && tail_items <= INT32_MAX / 16 && plan_tails(a, gp, r)) {
     r.items = tail_items;
-    r.arrive_at = r.own_at + up(2 * int64_t(sms) * r.warps * heads * (a.head_size * 4 + 8));
-    r.bytes = r.arrive_at + up(tail_items * 4);
+    const int64_t slot = heads * (a.head_size * 4 + 8), ranges = int64_t(sms) * r.warps;
+    r.own_at = up((items + sms) * r.tiles * int64_t(k.part_bytes));
+    r.found_at = r.own_at + up((tail_items + ranges) * slot);
+    r.bytes = r.found_at + up(tail_items * 8) + 256;
+    r.grid = sms;
+    const int64_t page = int64_t(a.head_size) * a.block_size * es * 2;  // bytes of a block and kv head
+    r.balance.sms = sms;
+    r.balance.prefix = units * 2600 * a.head_size / 128;
+    if (tune.prefix) r.balance.prefix = r.balance.prefix * tune.prefix / 100;
+    r.balance.block = page * 1000 / 65000;
+    r.balance.block_hbm = page * 1000 / 6500;
+    r.balance.prefix_start = 8000;
+    r.balance.behind_start = 14000;
   } else {
     // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
     r.items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
@@ -112,6 +128,7 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
     const int64_t tiles = (int64_t(std::max(a.max_seq_len - prefix_len, 1)) + 15) / 16;
     while (r.cluster < 8 && r.items * r.cluster * 10 <= places * 6 && r.cluster * kDirectWarps < tiles) r.cluster *= 2;
     if (tune.cluster) r.cluster = tune.cluster;
+    if (tune.behind == 2) r.cluster = 0;
   }
   r.k = k;
   return r;
@@ -183,8 +200,10 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   p.turns = plan.turns;
   p.scale = a->scale;
   if (plan.tails.fn != nullptr) {
-    p.arrive = reinterpret_cast<unsigned*>(p.parts + plan.arrive_at);
-    p.arrivals = int(plan.items);
+    p.cut = 0;
+    p.cut_out = reinterpret_cast<int*>(p.parts + plan.bytes - 256);
+    p.balance = plan.balance;
+    p.tail_items = int(plan.items / a->num_seqs);
   }
   cudaError_t e = plan.k.prefix(p, a->num_heads, plan.grid, s);
   count_launch();
@@ -231,15 +250,37 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
     d.use_table = 1;
     d.min_chunk = plan.min_chunk;
     pre.own = p.parts + plan.own_at;
-    pre.arrive = p.arrive;
+    pre.found = reinterpret_cast<int2*>(p.parts + plan.found_at);
+    pre.balance = plan.balance;
     e = plan.tails.fn(d, pre, sm_count(), plan.warps * 32, plan.smem, s);
   } else {
     d.head_groups = (p.group + plan.k.heads - 1) / plan.k.heads;
-    e = plan.k.behind(d, pre, int(plan.items), plan.cluster, s);
+    e = plan.cluster == 0 ? plan.k.solo(d, pre, int(plan.items), s)
+                          : plan.k.behind(d, pre, int(plan.items), plan.cluster, s);
   }
   count_launch();
   if (e != cudaSuccess) {
     set_error("shared prefix decode kernel launch failed: %s", cudaGetErrorString(e));
+    return B200PA_ECUDA;
+  }
+  if (plan.tails.fn == nullptr) return B200PA_OK;
+  CombineParams c{};
+  c.out = a->out;
+  c.v_scale = a->kv_dtype == B200PA_KV_AUTO ? nullptr : a->v_scale;
+  c.lse = a->out_lse;
+  c.cut = p.cut_out;
+  c.pre = pre;
+  c.num_seqs = a->num_seqs;
+  c.num_heads = a->num_heads;
+  c.group = p.group;
+  c.head_groups = d.head_groups;
+  c.heads = p.group <= 8 ? 8 : 16;
+  c.D = a->head_size;
+  e = launch_dependent(a->q_dtype == B200PA_BF16 ? shared_prefix_combine_kernel<__nv_bfloat16> : shared_prefix_combine_kernel<__half>,
+                       dim3(unsigned(plan.items)), dim3(kCombineThreads), 0, s, c);
+  count_launch();
+  if (e != cudaSuccess) {
+    set_error("shared prefix combine kernel launch failed: %s", cudaGetErrorString(e));
     return B200PA_ECUDA;
   }
   return B200PA_OK;

@@ -12,6 +12,8 @@ struct SharedPrefixKernels {
   cudaError_t (*prefix)(const SharedPrefixParams&, int num_heads, int grid, cudaStream_t stream) = nullptr;
   // what is behind it: `items` clusters
   cudaError_t (*behind)(const DecodeParams&, const SharedPrefixParts&, int items, int cluster, cudaStream_t stream) = nullptr;
+  // ... where a warp takes whole items
+  cudaError_t (*solo)(const DecodeParams&, const SharedPrefixParts&, int items, cudaStream_t stream) = nullptr;
   int heads = 0;        // query heads of an item of `behind`
   int ctas_per_sm = 0;  // of `behind`
   int row_tiles = 0;    // that share a K/V tile
@@ -59,16 +61,39 @@ cudaError_t behind_launch(const DecodeParams& p, const SharedPrefixParts& pre, i
   return launch_clusters<pa_decode_behind_kernel<QT, KV, D, GP>, DirectShape<KV, D, GP>::kSmem>(items, cluster, stream, p, pre);
 }
 
+template <typename QT, int KV, int D, int GP>
+cudaError_t solo_launch(const DecodeParams& p, const SharedPrefixParts& pre, int items, cudaStream_t stream) {
+  constexpr int smem = DirectShape<KV, D, GP>::kSmem;
+  auto kern = pa_decode_solo_kernel<QT, KV, D, GP>;
+  if constexpr (smem > 40 * 1024) {
+    static bool done[64] = {};
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && (dev < 0 || dev >= 64 || !done[dev])) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e == cudaSuccess && dev >= 0 && dev < 64) done[dev] = true;
+    }
+    if (e != cudaSuccess) {
+      (void)cudaGetLastError();
+      return e;
+    }
+  }
+  return launch_dependent(kern, dim3((items + kDirectWarps - 1) / kDirectWarps), dim3(kDirectWarps * 32), smem, stream, p, pre,
+                          items);
+}
+
 template <typename QT, int KV, int D>
 SharedPrefixKernels shared_prefix_kernels(int group) {
   SharedPrefixKernels k;
   k.prefix = shared_prefix_launch<QT, KV, D>;
   k.behind = behind_launch<QT, KV, D, 1>;
+  k.solo = solo_launch<QT, KV, D, 1>;
   k.heads = 8;
   k.ctas_per_sm = DirectShape<KV, D, 1>::kResident;
   if constexpr (D <= 128) {
     if (group > 8) {
       k.behind = behind_launch<QT, KV, D, 2>;
+      k.solo = solo_launch<QT, KV, D, 2>;
       k.heads = 16;
       k.ctas_per_sm = DirectShape<KV, D, 2>::kResident;
     }

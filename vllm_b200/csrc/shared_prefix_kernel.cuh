@@ -32,8 +32,6 @@ struct SharedPrefixParams {
   const float* alibi;
   const float* k_scale;
   unsigned char* parts;       // slots of one or two row tiles' parts
-  unsigned* arrive;           // counters of the launch behind, to be zeroed
-  int arrivals;
   int* status;
   int64_t q_stride;
   int64_t kv_block_stride;    // elements
@@ -46,7 +44,10 @@ struct SharedPrefixParams {
   int row_tiles;              // of a kv head
   int groups;                 // of row tiles of a kv head
   int key_tiles;              // of the prefix
-  int cut;                    // key tiles of a CTA
+  int cut;                    // key tiles of a CTA; 0: from `balance`
+  int* cut_out;               // where it is written then
+  SharedPrefixBalance balance;
+  int tail_items;             // (kv head, head group) pairs of a sequence behind the prefix
   int turns;                  // 1: one row tile, whose key tiles the warpgroups take in turns
   float scale;
 };
@@ -67,6 +68,7 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
   extern __shared__ __align__(1024) unsigned char smem[];
   __shared__ uint64_t s_bar[2 * NS + 14];
   __shared__ uint32_t s_tmem;
+  __shared__ int64_t s_blocks[kPrefillThreads / 32];
 
   const int tid = threadIdx.x, lane = tid & 31;
   const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);
@@ -80,6 +82,26 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
   auto q_full = [&](int i) { return bar0 + 8u * (2 * NS + 8 + i); };
   auto q_empty = [&](int i) { return bar0 + 8u * (2 * NS + 10 + i); };
   auto q_land = [&](int i) { return bar0 + 8u * (2 * NS + 12 + i); };
+
+  // (the launch behind this one may start now: it waits for this grid before it reads a part)
+  grid_dependency();
+  const int total = p.num_kv_heads * p.groups * p.key_tiles;
+  int cut = p.cut;
+  if (cut == 0) {  // SMs that are not needed here are the next launch's at once
+    int64_t blocks = 0;
+    for (int i = tid; i < p.num_seqs; i += kPrefillThreads)
+      blocks += work_units(max(__ldcg(p.seq_lens + i) - p.prefix_len, 0), p.block_size);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
+    if (lane == 0) s_blocks[warp] = blocks;
+    __syncthreads();
+    blocks = 0;
+    for (int w = 0; w < kPrefillThreads / 32; ++w) blocks += s_blocks[w];
+    const int ctas = p.balance.prefix_ctas(blocks * p.tail_items);
+    cut = (total + ctas - 1) / ctas;
+    if (blockIdx.x == 0 && tid == 0) *p.cut_out = cut;
+  }
+  if (int64_t(blockIdx.x) * cut >= total) return;
 
   const uint32_t sq = smem_u32(smem);
   const uint32_t skv = sq + NQ * SH::kQBytes;
@@ -119,9 +141,6 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  // (the launch behind this one may start now: it waits for this grid before it reads a part)
-  grid_dependency();
-  for (int i = blockIdx.x * kPrefillThreads + tid; i < p.arrivals; i += gridDim.x * kPrefillThreads) p.arrive[i] = 0;
 
   const int G = p.group, B = p.block_size, b_shift = 31 - __clz(B);
   const int T = 128 / G;  // sequences of a row tile
@@ -131,9 +150,8 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
     int item, kvh, tile0;  // tile0: first row tile
     int b, e;              // key tiles
   };
-  const int total = p.num_kv_heads * p.groups * p.key_tiles;
-  const int u_end = min(total, (int(blockIdx.x) + 1) * p.cut);
-  int u = int(blockIdx.x) * p.cut;
+  const int u_end = min(total, (int(blockIdx.x) + 1) * cut);
+  int u = int(blockIdx.x) * cut;
   auto next = [&](Piece& it) -> bool {
     if (u >= u_end) return false;
     it.item = u / p.key_tiles;
@@ -673,6 +691,113 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
   if (warp == 12) {
     tc_fence_after();
     tmem_dealloc(tmem, 512);
+  }
+}
+
+// The sum of all parts of a sequence: a CTA to an item, a thread to four dimensions of a head, or several that share
+// the parts between them where there are threads to spare.
+constexpr int kCombineThreads = 256;
+
+struct CombineParams {
+  void* out;
+  const float* v_scale;  // nullptr: 1
+  float* lse;
+  const int* cut;
+  SharedPrefixParts pre;
+  int num_seqs, num_heads, group, head_groups, heads, D;  // heads: of an item
+};
+
+template <typename QT>
+__global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(const CombineParams p) {
+  constexpr bool kBf = std::is_same_v<QT, __nv_bfloat16>;
+  __shared__ float4 s_acc[kCombineThreads];
+  __shared__ float2 s_ml[kCombineThreads];
+  grid_dependency();
+  const int tid = threadIdx.x, D = p.D, HPI = p.heads;
+  const int seq = blockIdx.x % p.num_seqs, sub = blockIdx.x / p.num_seqs;
+  const int kvh = sub / p.head_groups, hg = sub - kvh * p.head_groups;
+  const int nheads = min(HPI, p.group - hg * HPI), units = nheads * (D / 4);
+  const int cut = __ldcg(p.cut);
+  const int2 found = __ldcg(p.pre.found + blockIdx.x);
+  const int64_t own_slot = int64_t(HPI) * (D * 4 + 8), part = 128 * (D * 4 + 8);
+  const unsigned char* own = p.pre.own + (int64_t(blockIdx.x) + found.x) * own_slot;
+  // (SharedPrefixParts::row, with the cut that the prefix's kernel has chosen)
+  const int tile = seq / p.pre.tokens, grp = p.pre.turns ? tile : tile / p.pre.tiles;
+  const int64_t it = int64_t(kvh) * p.pre.groups + grp, u0 = it * p.pre.key_tiles;
+  const int c0 = int(u0 / cut), c1 = int((u0 + p.pre.key_tiles - 1) / cut);
+  const unsigned char* first =
+      p.pre.parts + ((it + c0) * p.pre.tiles + (p.pre.turns ? 0 : tile - grp * p.pre.tiles)) * part;
+  const int64_t step = p.pre.turns ? part : p.pre.tiles * part;
+  const int row = (seq - tile * p.pre.tokens) * p.group + hg * HPI;
+  const int np = found.y, n = np + (c1 - c0 + 1) * (p.pre.turns ? 2 : 1);
+  const float v_scale = p.v_scale ? __ldcg(p.v_scale) : 1.f;
+
+  // threads that share a unit: 1, 2, 4 ...
+  int share = 1;
+  while (share * 2 * units <= kCombineThreads && share * 4 < n) share *= 2;
+  const int lanes = kCombineThreads / share;
+  for (int u0 = 0; u0 < units; u0 += lanes) {
+    const int u = u0 + tid % lanes, z = tid / lanes;
+    const bool on = u < units;
+    const int hl = on ? u % nheads : 0, d4 = on ? u / nheads : 0;
+    float m = -INFINITY, l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = z; k0 < n && on; k0 += 4 * share) {
+      float2 ml[4];
+      float4 v[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int s = min(k0 + k * share, n - 1);
+        const unsigned char* q = s < np ? own + s * own_slot : first + (s - np) * step;
+        ml[k] = __ldcg(reinterpret_cast<const float2*>(s < np ? q + HPI * D * 4 + hl * 8 : q + 128 * D * 4 + (row + hl) * 8));
+        v[k] = __ldcg(reinterpret_cast<const float4*>(s < np ? q + (d4 * HPI + hl) * 16 : q + (d4 * 128 + row + hl) * 16));
+        if (k0 + k * share >= n) ml[k] = make_float2(-INFINITY, 0.f);
+      }
+      float m_new = m;
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (ml[k].y != 0.f) m_new = fmaxf(m_new, ml[k].x);
+      const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new);
+      l *= old;
+      acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+      m = m_new;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if (ml[k].y != 0.f) {  // (what has no key has written no output)
+          const float f = fast_exp2(ml[k].x - m);
+          l += ml[k].y * f;
+          acc.x += f * v[k].x;
+          acc.y += f * v[k].y;
+          acc.z += f * v[k].z;
+          acc.w += f * v[k].w;
+        }
+      }
+    }
+    if (share > 1) {  // (one pass then: every unit has its threads)
+      s_acc[tid] = acc;
+      s_ml[tid] = make_float2(m, l);
+      __syncthreads();
+      if (z > 0 || !on) continue;
+      for (int k = 1; k < share; ++k) {
+        const float2 ml = s_ml[tid + k * lanes];
+        if (ml.y == 0.f) continue;
+        const float4 v = s_acc[tid + k * lanes];
+        const float m_new = fmaxf(m, ml.x);
+        const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new), f = fast_exp2(ml.x - m_new);
+        l = l * old + ml.y * f;
+        acc = make_float4(acc.x * old + v.x * f, acc.y * old + v.y * f, acc.z * old + v.z * f, acc.w * old + v.w * f);
+        m = m_new;
+      }
+    }
+    if (!on) continue;
+    const float inv = v_scale * __fdividef(1.f, l + 1e-6f);
+    const int head = kvh * p.group + hg * HPI + hl;
+    uint2 w;
+    w.x = pack2<kBf>(acc.x * inv, acc.y * inv);
+    w.y = pack2<kBf>(acc.z * inv, acc.w * inv);
+    *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + head) * D + d4 * 4) = w;
+    if (p.lse != nullptr && d4 == 0)
+      p.lse[int64_t(head) * p.num_seqs + seq] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
 }
 
