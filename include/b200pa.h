@@ -227,19 +227,26 @@ int b200pa_paged_attention_varlen_supported(const b200pa_attn_args* args);
 
 /*
  * Decode attention of a batch whose sequences begin with the same `prefix_len` tokens, in the same cache
- * blocks: those of block_tables[0], whatever the first prefix_len / block_size entries of the other rows say
- * (where they say the same, the result is that of paged_attention_v1, but for rounding).  K and V of the
- * prefix are read once for the whole batch.  No counterpart in the reference's paged-attention ops.
+ * blocks: every row of block_tables begins with them.  The result is that of paged_attention_v1, but for
+ * rounding; K and V of the prefix are read once for the whole batch.  (That the rows agree is not checked: the
+ * prefix is read through row 0, or through every row where the call runs as paged_attention_v1.)  No counterpart in
+ * the reference's paged-attention ops.
  *   args: as for v1 (out_lse included; seq_lens, max_seq_len and the block tables cover prefix and own tokens);
  *     block-sparse arguments are not supported.  A sequence shorter than the prefix sees the keys that it has.
  *   prefix_len: a multiple of block_size, 0 included
  *   scratch: device memory on a 16-byte boundary, of b200pa_shared_prefix_scratch_bytes bytes at least; its
  *     contents do not matter, and nothing else is kept between calls: calls with scratch of their own may overlap
- * Shapes that have no kernel for the prefix (fp32 queries, block size 8, unaligned tensors, a single sequence) run
- * as paged_attention_v1 on the whole sequences and need no scratch.
+ * Shapes that have no kernel for the prefix (fp32 queries, block size 8, unaligned tensors, a single sequence), and
+ * batches with too little to share, run as paged_attention_v1 on the whole sequences and need no scratch.
  */
 int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args, int32_t prefix_len, void* scratch,
                                          int64_t scratch_bytes, void* stream);
+
+/* Which kernels a call of these sizes, types, strides and alignments runs on, with own parts of up to
+ * max_seq_len - prefix_len tokens; launches nothing and reads no tensor.  *way: 0 as paged_attention_v1; else the
+ * prefix's kernel, and behind it 1 the direct decode kernel, 2 the same with a warp to every (sequence, kv head, head
+ * group), 3 the persistent one, which runs beside the prefix, and a launch that adds up. */
+int b200pa_shared_prefix_route(const b200pa_attn_args* args, int32_t prefix_len, int32_t* way);
 
 /* Bytes of scratch that the call needs on the current device (sizes, types, strides and alignments of `args`
  * count, no tensor is read); 0: none; a negative B200PA_E* code: what the call is refused for. */

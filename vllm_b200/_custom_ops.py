@@ -305,11 +305,12 @@ def paged_attention_shared_prefix(
     lse: torch.Tensor | None = None,
 ) -> None:
     """``paged_attention_v1`` for a batch whose sequences begin with the same `prefix_len` tokens (a
-    multiple of the block size) in the same blocks, those of ``block_tables[0]``: K and V of the prefix
-    are read once for all sequences.  Lengths and block tables cover prefix and own tokens; a sequence
+    multiple of the block size) in the same blocks, with which every row of `block_tables` begins (not
+    checked): K and V of the prefix are read once for all sequences.  Lengths and block tables cover prefix and own tokens; a sequence
     shorter than the prefix sees the keys that it has.  `lse` [num_heads, num_seqs] (float32), where
     given, is filled as by ``paged_attention_with_lse``.  Shapes without a kernel for the prefix (fp32,
-    block size 8, unaligned tensors, one sequence) run as ``paged_attention_v1``."""
+    block size 8, unaligned tensors, one sequence), and batches with too little to share, run as
+    ``paged_attention_v1``."""
     if not _compiling() and _direct.paged_attention_shared_prefix(
             out, query, key_cache, value_cache, num_kv_heads, scale, block_tables, seq_lens, prefix_len,
             block_size, max_seq_len, alibi_slopes, kv_cache_dtype, k_scale, v_scale, lse):

@@ -25,6 +25,7 @@ EXPORTS = (
     "b200pa_reshape_and_cache_flash",
     "b200pa_paged_attention_shared_prefix",
     "b200pa_shared_prefix_scratch_bytes",
+    "b200pa_shared_prefix_route",
     "b200pa_rotary_reshape_and_cache",
     "b200pa_rotary_reshape_and_cache_flash",
     "b200pa_paged_attention_varlen",
@@ -108,6 +109,7 @@ def lib() -> C.CDLL:
                                                            C.c_void_p]
         l.b200pa_shared_prefix_scratch_bytes.argtypes = [C.POINTER(AttnArgs), C.c_int32]
         l.b200pa_shared_prefix_scratch_bytes.restype = C.c_int64
+        l.b200pa_shared_prefix_route.argtypes = [C.POINTER(AttnArgs), C.c_int32, C.POINTER(C.c_int32)]
         l.b200pa_convert_fp8.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_float, C.c_int32,
                                          C.c_int32, C.c_int32, C.c_void_p]
         l.b200pa_decode_route.argtypes = [C.POINTER(AttnArgs), C.POINTER(C.c_int32)]
@@ -159,6 +161,13 @@ def reshape_and_cache(args: CacheArgs, stream: int = 0) -> None:
 
 def reshape_and_cache_flash(args: CacheArgs, stream: int = 0) -> None:
     check(lib().b200pa_reshape_and_cache_flash(C.byref(args), C.c_void_p(stream)))
+
+
+def shared_prefix_route(args: AttnArgs, prefix_len: int) -> int:
+    """Which kernels a call runs on (see b200pa.h); 0: as paged_attention_v1."""
+    v = C.c_int32(0)
+    check(lib().b200pa_shared_prefix_route(C.byref(args), prefix_len, C.byref(v)))
+    return v.value
 
 
 def shared_prefix_scratch_bytes(args: AttnArgs, prefix_len: int) -> int:

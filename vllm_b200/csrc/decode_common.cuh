@@ -64,6 +64,7 @@ struct SharedPrefixBalance {
   int64_t prefix;        // of one SM, in all
   int64_t block;         // of one SM, per cache block of one item behind the prefix
   int64_t block_hbm;     // of all SMs, in thousandths: what HBM takes at least
+  int64_t items;         // of one SM, for all items behind it, beside their blocks
   int64_t prefix_start;  // before and behind the work itself
   int64_t behind_start;
   int sms;
@@ -73,7 +74,7 @@ struct SharedPrefixBalance {
     while (lo < hi) {
       const int g = (lo + hi) >> 1;
       const int64_t tp = prefix_start + prefix / g;
-      const int64_t tb = behind_start + max(blocks * block / (sms - g), blocks * block_hbm / 1000);
+      const int64_t tb = behind_start + max((blocks * block + items) / (sms - g), blocks * block_hbm / 1000);
       if (tp <= tb) hi = g; else lo = g + 1;
     }
     return lo;

@@ -1,5 +1,6 @@
 // Host entry of decode attention over a prefix that all sequences of the batch share.
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 
 #include "launch_state.cuh"
@@ -18,6 +19,7 @@ struct SharedPrefixPlan {
   int warps = 0, slots = 0, min_chunk = 0;
   size_t smem = 0;
   int cluster = 1;  // 0: every warp an item of its own
+  int heads = 0;                                // query heads of an item of the persistent kernel
   int64_t items = 0;                            // (sequence, kv head, head group)
   SharedPrefixBalance balance{};
   int64_t own_at = 0, found_at = 0, bytes = 0;  // scratch: the prefix's parts, partials, their places; its size
@@ -80,6 +82,45 @@ static SharedPrefixKernels find_shared_prefix(const b200pa_attn_args& a) {
                               : find_shared_prefix_large(a.head_size, a.q_dtype, a.kv_dtype, group);
 }
 
+// What the prefix's kernel takes for a key tile of an item, ns of an SM: two row tiles in turns on the tensor cores, or
+// one by itself (measured: 128 fp8 sequences, 64 / 8 heads of 128, behind 8192 2.3 us; 8 sequences behind 65008 1.55;
+// head sizes 64 and 256 2.0 and 1.8), or its K and V on the way.
+static int64_t unit_ns(int head_size, int row_tiles, int turns, int64_t tile_bytes) {
+  const int64_t work = row_tiles == 1 ? 1800 : turns ? 1000 + 4 * head_size : 1500 + 8 * std::min(head_size, 128);
+  return std::max(work, tile_bytes * 1000 / 60000);
+}
+
+// Which way a call goes: 0 the ordinary kernels on whole sequences; behind the prefix the direct kernel (1), the same
+// with a warp to an item (2), or the persistent one beside the prefix and a third launch (3).  What each takes, us:
+// fitted to 260 random batches (2 to 2000 sequences, prefixes of 64 to 65000 tokens, up to 3000 own ones, all head sizes,
+// cache types and ten head counts; own lengths are taken as half the bound).  The choice is 3 % from the best of the four
+// on average, more than 25 % in 9 cases; each of them alone 82, 21, 85 and 50 %.
+//   prefix_all: the prefix's work over all SMs; prefix_cut: of its longest CTA
+static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const SharedPrefixPlan& r, double prefix_all,
+                             double prefix_cut, bool tails) {
+  const int group = a.num_heads / a.num_kv_heads, es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1, sms = sm_count();
+  const double D = a.head_size, N = a.num_seqs, us = 1 / 6.5e6;  // (bytes to us at HBM's rate)
+  const double own = std::max(a.max_seq_len - prefix_len, 1), tiles = own / 16 + 0.5;
+  const double row = a.num_kv_heads * D * 2 * es, hbm = N * own / 2 * row * us;
+  const double latency = (es == 1 ? 0.63 + 0.0037 * D : 0.43 + 0.0061 * D) * (group > 8 ? 1.4 : 1);  // of a tile
+  const double prefix = 8 + prefix_cut, places = 3.0 * sms, warps = r.cluster * kDirectWarps, items = double(r.items);
+  const double waves = std::max(1.0, items * r.cluster / places), solo_waves = std::max(1.0, items / places / kDirectWarps);
+  // trips to the prefix's parts, of which a row of few sequences has over a hundred
+  const double parts = (double(r.key_tiles) / r.cut + 1) * (r.turns ? 2 : 1);
+  const double rounds = std::ceil(parts / (4 * r.cluster)) * std::ceil(std::min(group, 16) * D / 4 / 128);
+  double t[4];
+  t[0] = 14.6 + 1.24 * N * (prefix_len + own / 2) * row * us;
+  t[1] = prefix + 6 + std::max({1.2 * hbm, 1.9 * tiles / warps * latency,
+                                waves * (2.6 + std::max(own / 32 / warps, 0.5) * latency)}) +
+         0.8 * std::max(rounds - 4, 0.0);
+  t[2] = prefix + 5 + std::max({1.2 * hbm, 0.9 * tiles * latency, solo_waves * (3.4 + std::max(own / 32, 1.0) * latency)}) +
+         0.8 * std::max(parts - 8, 0.0);
+  const double tail_items = N * a.num_kv_heads * ((group + (group <= 8 ? 7 : 15)) / (group <= 8 ? 8 : 16));
+  const double beside = (N * own / 2 * row / 65e3 + tail_items * 0.5) / sms;
+  t[3] = tails ? 31 + std::max(prefix_all + beside, hbm) + 0.7e-6 * N * a.num_heads * D * 4 : 1e30;
+  return int(std::min_element(t, t + 4) - t);
+}
+
 static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix_len) {
   SharedPrefixPlan r;
   if (a.num_seqs < 2 || prefix_len == 0) return r;
@@ -105,8 +146,22 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   // ---- behind the prefix
   const int gp = group <= 8 ? 1 : 2, heads = 8 * gp;
   const int64_t tail_items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + heads - 1) / heads);
-  if (tune.behind == 3 && tail_items <= INT32_MAX / 16 && plan_tails(a, gp, r)) {
+  r.items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
+  if (r.items > INT32_MAX / 16) return r;
+  const int64_t unit = unit_ns(a.head_size, k.row_tiles, r.turns, int64_t(k.keys) * a.head_size * 2 * es);
+  const int64_t places = int64_t(sms) * k.ctas_per_sm;
+  const int64_t own_tiles = (int64_t(std::max(a.max_seq_len - prefix_len, 1)) + 15) / 16;
+  // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
+  while (r.cluster < 8 && r.items * r.cluster * 10 <= places * 6 && r.cluster * kDirectWarps < own_tiles) r.cluster *= 2;
+  if (tune.cluster) r.cluster = tune.cluster;
+  const bool tails = tail_items <= INT32_MAX / 16 && plan_tails(a, gp, r);
+  const int way = tune.behind ? tune.behind : shared_prefix_way(a, prefix_len, r, units * unit * 1e-3 / sms, r.cut * unit * 1e-3, tails);
+  if (way == 0) return r;
+  if (way != 3) r.tails.fn = nullptr;
+  if (way == 2) r.cluster = 0;
+  if (r.tails.fn != nullptr) {
     r.items = tail_items;
+    r.heads = heads;
     const int64_t slot = heads * (a.head_size * 4 + 8), ranges = int64_t(sms) * r.warps;
     r.own_at = up((items + sms) * r.tiles * int64_t(k.part_bytes));
     r.found_at = r.own_at + up((tail_items + ranges) * slot);
@@ -114,21 +169,13 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
     r.grid = sms;
     const int64_t page = int64_t(a.head_size) * a.block_size * es * 2;  // bytes of a block and kv head
     r.balance.sms = sms;
-    r.balance.prefix = units * 2600 * a.head_size / 128;
+    r.balance.prefix = units * unit;
+    r.balance.items = tail_items * 500;
     if (tune.prefix) r.balance.prefix = r.balance.prefix * tune.prefix / 100;
     r.balance.block = page * 1000 / 65000;
     r.balance.block_hbm = page * 1000 / 6500;
     r.balance.prefix_start = 8000;
     r.balance.behind_start = 14000;
-  } else {
-    // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
-    r.items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
-    if (r.items > INT32_MAX / 16) return r;
-    const int64_t places = int64_t(sms) * k.ctas_per_sm;
-    const int64_t tiles = (int64_t(std::max(a.max_seq_len - prefix_len, 1)) + 15) / 16;
-    while (r.cluster < 8 && r.items * r.cluster * 10 <= places * 6 && r.cluster * kDirectWarps < tiles) r.cluster *= 2;
-    if (tune.cluster) r.cluster = tune.cluster;
-    if (tune.behind == 2) r.cluster = 0;
   }
   r.k = k;
   return r;
@@ -152,6 +199,15 @@ static b200pa_attn_args with_plain_strides(b200pa_attn_args a) {
 }
 
 }  // namespace b200pa
+
+extern "C" int b200pa_shared_prefix_route(const b200pa_attn_args* args, int32_t prefix_len, int32_t* way) {
+  using namespace b200pa;
+  B200PA_CHECK_ARG(way != nullptr, "way is NULL");
+  if (const int bad = check_shared_prefix(args, prefix_len); bad != B200PA_OK) return bad;
+  const SharedPrefixPlan plan = args->num_seqs > 0 ? shared_prefix_plan(with_plain_strides(*args), prefix_len) : SharedPrefixPlan{};
+  *way = plan.k.prefix == nullptr ? 0 : plan.tails.fn != nullptr ? 3 : plan.cluster == 0 ? 2 : 1;
+  return B200PA_OK;
+}
 
 extern "C" int64_t b200pa_shared_prefix_scratch_bytes(const b200pa_attn_args* args, int32_t prefix_len) {
   using namespace b200pa;
@@ -245,7 +301,7 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   pre.tiles = plan.tiles;
   pre.turns = plan.turns;
   if (plan.tails.fn != nullptr) {
-    d.head_groups = (p.group + (p.group <= 8 ? 8 : 16) - 1) / (p.group <= 8 ? 8 : 16);
+    d.head_groups = (p.group + plan.heads - 1) / plan.heads;
     d.nstages = plan.slots;
     d.use_table = 1;
     d.min_chunk = plan.min_chunk;
@@ -274,10 +330,16 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   c.num_heads = a->num_heads;
   c.group = p.group;
   c.head_groups = d.head_groups;
-  c.heads = p.group <= 8 ? 8 : 16;
+  c.heads = plan.heads;
+  // threads that share four dimensions of a head: 1, 2, 4 ... 32, so that each adds up a few parts
+  const int64_t most = int64_t(plan.key_tiles) * p.num_kv_heads * plan.groups < sm_count() ? plan.key_tiles
+                       : sm_count() / (p.num_kv_heads * plan.groups) + 2;
+  c.share = 1;
+  while (c.share < 32 && c.share * 6 < most * (plan.turns ? 2 : 1)) c.share *= 2;
+  const int lanes = kCombineThreads / c.share, per_item = std::min(p.group, plan.heads) * (a->head_size / 4);
   c.D = a->head_size;
   e = launch_dependent(a->q_dtype == B200PA_BF16 ? shared_prefix_combine_kernel<__nv_bfloat16> : shared_prefix_combine_kernel<__half>,
-                       dim3(unsigned(plan.items)), dim3(kCombineThreads), 0, s, c);
+                       dim3(unsigned(plan.items), unsigned((per_item + lanes - 1) / lanes)), dim3(kCombineThreads), 0, s, c);
   count_launch();
   if (e != cudaSuccess) {
     set_error("shared prefix combine kernel launch failed: %s", cudaGetErrorString(e));

@@ -694,8 +694,8 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
   }
 }
 
-// The sum of all parts of a sequence: a CTA to an item, a thread to four dimensions of a head, or several that share
-// the parts between them where there are threads to spare.
+// The sum of all parts of a sequence: grid.x = items, a thread to four dimensions of a head, or several, which share the
+// parts between them (few sequences behind a long prefix have over a hundred).
 constexpr int kCombineThreads = 256;
 
 struct CombineParams {
@@ -705,6 +705,7 @@ struct CombineParams {
   const int* cut;
   SharedPrefixParts pre;
   int num_seqs, num_heads, group, head_groups, heads, D;  // heads: of an item
+  int share;                                              // threads to a unit
 };
 
 template <typename QT>
@@ -732,73 +733,68 @@ __global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(
   const int np = found.y, n = np + (c1 - c0 + 1) * (p.pre.turns ? 2 : 1);
   const float v_scale = p.v_scale ? __ldcg(p.v_scale) : 1.f;
 
-  // threads that share a unit: 1, 2, 4 ...
-  int share = 1;
-  while (share * 2 * units <= kCombineThreads && share * 4 < n) share *= 2;
-  const int lanes = kCombineThreads / share;
-  for (int u0 = 0; u0 < units; u0 += lanes) {
-    const int u = u0 + tid % lanes, z = tid / lanes;
-    const bool on = u < units;
-    const int hl = on ? u % nheads : 0, d4 = on ? u / nheads : 0;
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = z; k0 < n && on; k0 += 4 * share) {
-      float2 ml[4];
-      float4 v[4];
+  const int share = p.share, lanes = kCombineThreads / share;
+  const int u = blockIdx.y * lanes + tid % lanes, z = tid / lanes;
+  const bool on = u < units;
+  const int hl = on ? u % nheads : 0, d4 = on ? u / nheads : 0;
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int k0 = z; k0 < n && on; k0 += 4 * share) {
+    float2 ml[4];
+    float4 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int s = min(k0 + k * share, n - 1);
-        const unsigned char* q = s < np ? own + s * own_slot : first + (s - np) * step;
-        ml[k] = __ldcg(reinterpret_cast<const float2*>(s < np ? q + HPI * D * 4 + hl * 8 : q + 128 * D * 4 + (row + hl) * 8));
-        v[k] = __ldcg(reinterpret_cast<const float4*>(s < np ? q + (d4 * HPI + hl) * 16 : q + (d4 * 128 + row + hl) * 16));
-        if (k0 + k * share >= n) ml[k] = make_float2(-INFINITY, 0.f);
-      }
-      float m_new = m;
+    for (int k = 0; k < 4; ++k) {
+      const int s = min(k0 + k * share, n - 1);
+      const unsigned char* q = s < np ? own + s * own_slot : first + (s - np) * step;
+      ml[k] = __ldcg(reinterpret_cast<const float2*>(s < np ? q + HPI * D * 4 + hl * 8 : q + 128 * D * 4 + (row + hl) * 8));
+      v[k] = __ldcg(reinterpret_cast<const float4*>(s < np ? q + (d4 * HPI + hl) * 16 : q + (d4 * 128 + row + hl) * 16));
+      if (k0 + k * share >= n) ml[k] = make_float2(-INFINITY, 0.f);
+    }
+    float m_new = m;
 #pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (ml[k].y != 0.f) m_new = fmaxf(m_new, ml[k].x);
-      const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new);
-      l *= old;
-      acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
-      m = m_new;
+    for (int k = 0; k < 4; ++k)
+      if (ml[k].y != 0.f) m_new = fmaxf(m_new, ml[k].x);
+    const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new);
+    l *= old;
+    acc = make_float4(acc.x * old, acc.y * old, acc.z * old, acc.w * old);
+    m = m_new;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        if (ml[k].y != 0.f) {  // (what has no key has written no output)
-          const float f = fast_exp2(ml[k].x - m);
-          l += ml[k].y * f;
-          acc.x += f * v[k].x;
-          acc.y += f * v[k].y;
-          acc.z += f * v[k].z;
-          acc.w += f * v[k].w;
-        }
+    for (int k = 0; k < 4; ++k) {
+      if (ml[k].y != 0.f) {  // (what has no key has written no output)
+        const float f = fast_exp2(ml[k].x - m);
+        l += ml[k].y * f;
+        acc.x += f * v[k].x;
+        acc.y += f * v[k].y;
+        acc.z += f * v[k].z;
+        acc.w += f * v[k].w;
       }
     }
-    if (share > 1) {  // (one pass then: every unit has its threads)
-      s_acc[tid] = acc;
-      s_ml[tid] = make_float2(m, l);
-      __syncthreads();
-      if (z > 0 || !on) continue;
-      for (int k = 1; k < share; ++k) {
-        const float2 ml = s_ml[tid + k * lanes];
-        if (ml.y == 0.f) continue;
-        const float4 v = s_acc[tid + k * lanes];
-        const float m_new = fmaxf(m, ml.x);
-        const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new), f = fast_exp2(ml.x - m_new);
-        l = l * old + ml.y * f;
-        acc = make_float4(acc.x * old + v.x * f, acc.y * old + v.y * f, acc.z * old + v.z * f, acc.w * old + v.w * f);
-        m = m_new;
-      }
-    }
-    if (!on) continue;
-    const float inv = v_scale * __fdividef(1.f, l + 1e-6f);
-    const int head = kvh * p.group + hg * HPI + hl;
-    uint2 w;
-    w.x = pack2<kBf>(acc.x * inv, acc.y * inv);
-    w.y = pack2<kBf>(acc.z * inv, acc.w * inv);
-    *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + head) * D + d4 * 4) = w;
-    if (p.lse != nullptr && d4 == 0)
-      p.lse[int64_t(head) * p.num_seqs + seq] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
   }
+  if (share > 1) {
+    s_acc[tid] = acc;
+    s_ml[tid] = make_float2(m, l);
+    __syncthreads();
+    if (z > 0 || !on) return;
+    for (int k = 1; k < share; ++k) {
+      const float2 ml = s_ml[tid + k * lanes];
+      if (ml.y == 0.f) continue;
+      const float4 v = s_acc[tid + k * lanes];
+      const float m_new = fmaxf(m, ml.x);
+      const float old = m_new == -INFINITY ? 0.f : fast_exp2(m - m_new), f = fast_exp2(ml.x - m_new);
+      l = l * old + ml.y * f;
+      acc = make_float4(acc.x * old + v.x * f, acc.y * old + v.y * f, acc.z * old + v.z * f, acc.w * old + v.w * f);
+      m = m_new;
+    }
+  }
+  if (!on) return;
+  const float inv = v_scale * __fdividef(1.f, l + 1e-6f);
+  const int head = kvh * p.group + hg * HPI + hl;
+  uint2 w;
+  w.x = pack2<kBf>(acc.x * inv, acc.y * inv);
+  w.y = pack2<kBf>(acc.z * inv, acc.w * inv);
+  *reinterpret_cast<uint2*>(static_cast<QT*>(p.out) + (int64_t(seq) * p.num_heads + head) * D + d4 * 4) = w;
+  if (p.lse != nullptr && d4 == 0)
+    p.lse[int64_t(head) * p.num_seqs + seq] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
 }
 
 }  // namespace b200pa
