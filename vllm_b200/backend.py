@@ -46,6 +46,7 @@ class B200PagedAttentionMetadata:
     slot_mapping: torch.Tensor      # [num_tokens] int64, cache slot of every new token
     use_cascade: bool = False
     num_decodes: int = 0            # requests in front of the batch that bring exactly one token
+    common_prefix_len: int = 0      # tokens that all requests begin with, in the same blocks (cascade)
 
 
 def leading_decodes(query_start_loc_cpu: torch.Tensor | None) -> int:
@@ -107,13 +108,17 @@ class B200PagedAttentionMetadataBuilder:
     def get_cudagraph_support(cls, vllm_config=None, kv_cache_spec=None):
         return cls._cudagraph_support
 
+    def use_cascade_attention(self, *args, **kwargs) -> bool:
+        return B200PagedAttentionBackend.use_cascade_attention(*args, **kwargs)
+
     def build(self, common_prefix_len: int, common_attn_metadata,
               fast_build: bool = False) -> B200PagedAttentionMetadata:
-        if common_prefix_len > 0:
-            raise NotImplementedError("cascade attention is not supported by the paged-attention ops "
-                                      "(use_cascade_attention() returns False)")
         m = common_attn_metadata
+        if common_prefix_len % self.block_size != 0 or common_prefix_len > m.max_seq_len:
+            raise NotImplementedError(f"a common prefix has to be whole blocks of {self.block_size} tokens that every "
+                                      f"request has: got {common_prefix_len} tokens")
         return B200PagedAttentionMetadata(
+            use_cascade=common_prefix_len > 0, common_prefix_len=common_prefix_len,
             num_actual_tokens=m.num_actual_tokens, max_query_len=m.max_query_len,
             query_start_loc=m.query_start_loc, max_seq_len=m.max_seq_len, seq_lens=m.seq_lens,
             block_table=m.block_table_tensor, slot_mapping=m.slot_mapping,
@@ -155,21 +160,36 @@ class B200PagedAttentionImpl:
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
         self.num_queries_per_kv = num_heads // num_kv_heads
 
-    def forward(self, layer, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+    def fused_rope_kvcache_supported(self) -> bool:
+        return self.kv_sharing_target_layer_name is None
+
+    def do_rope_and_kv_cache_update(self, layer, query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                                    positions: torch.Tensor, cos_sin_cache: torch.Tensor, is_neox: bool,
+                                    kv_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+        """Rotates `query` in place and writes the rotated `key` and `value` to the cache, in one launch
+        (``rotary_reshape_and_cache``); `key` stays as it is.  `forward` is called with ``key`` and
+        ``value`` None then."""
+        key_cache, value_cache = PagedAttention.split_kv_cache(kv_cache, self.num_kv_heads, self.head_size)
+        PagedAttention.rotate_and_write_to_paged_cache(
+            query, key, value, positions, cos_sin_cache, is_neox, key_cache, value_cache, slot_mapping,
+            self.kv_cache_dtype, layer._k_scale, layer._v_scale, query_out=query)
+
+    def forward(self, layer, query: torch.Tensor, key: torch.Tensor | None, value: torch.Tensor | None,
                 kv_cache: torch.Tensor, attn_metadata: B200PagedAttentionMetadata | None,
                 output: torch.Tensor | None = None, output_scale=None,
                 output_block_scale=None) -> torch.Tensor:
         """query [num_tokens, num_heads, head_size]; key/value [num_tokens, num_kv_heads,
-        head_size]; kv_cache [2, num_blocks, block_size * num_kv_heads * head_size];
-        `layer` carries `_k_scale` / `_v_scale` float32 tensors.  Returns `output`."""
+        head_size], or None where the cache has them already; kv_cache [2, num_blocks, block_size *
+        num_kv_heads * head_size]; `layer` carries `_k_scale` / `_v_scale` float32 tensors.  Returns `output`."""
         assert output is not None, "Output tensor must be provided."
         if output_scale is not None or output_block_scale is not None:
             raise NotImplementedError("fused output quantisation is not supported")
         if attn_metadata is None:  # profiling run
             return output.fill_(0)
         md = attn_metadata
-        assert md.use_cascade is False
         n = md.num_actual_tokens
+        assert (key is None) == (value is None), "key and value go together"
+        write = key is not None and self.kv_sharing_target_layer_name is None
         alibi = self.alibi_slopes
         if alibi is not None and alibi.device != query.device:
             alibi = self.alibi_slopes = alibi.to(query.device)
@@ -179,37 +199,46 @@ class B200PagedAttentionImpl:
         num_decodes = md.num_decodes
         if md.max_query_len > 1 and torch.cuda.is_current_stream_capturing():
             num_decodes = 0
-        if ops.attention_step(
+        cascade = md.use_cascade and num_decodes > 1
+        if not cascade and ops.attention_step(
                 output, query, key, value, kv_cache, md.block_table, md.seq_lens, md.slot_mapping,
                 md.query_start_loc, layer._k_scale, layer._v_scale, alibi, n, num_decodes,
                 md.max_query_len, md.max_seq_len, self.num_heads, self.num_kv_heads, self.head_size,
-                self.scale, self.kv_cache_dtype, self.kv_sharing_target_layer_name is None,
+                self.scale, self.kv_cache_dtype, write,
                 PagedAttention.use_v1(md.max_seq_len, n, self.num_heads)):
             return output
-        # not a plain call (fp32, odd strides, tracing, ...): operator by operator
+        # a cascade step, or not a plain call (fp32, odd strides, tracing, ...): operator by operator
         key_cache, value_cache = PagedAttention.split_kv_cache(kv_cache, self.num_kv_heads,
                                                                self.head_size)
-        if self.kv_sharing_target_layer_name is None:
+        if write:
             PagedAttention.write_to_paged_cache(key[:n], value[:n], key_cache, value_cache,
                                                 attn_metadata.slot_mapping[:n], self.kv_cache_dtype,
                                                 layer._k_scale, layer._v_scale)
         q = query[:n].view(n, self.num_heads, self.head_size)
-        if attn_metadata.max_query_len == 1:
-            seq_lens, block_table = attn_metadata.seq_lens, attn_metadata.block_table
-        elif ops.paged_attention_varlen(
-                output[:n].view(n, self.num_heads, self.head_size), q, key_cache, value_cache,
-                self.num_kv_heads, self.scale, attn_metadata.block_table, attn_metadata.seq_lens,
-                attn_metadata.query_start_loc, num_decodes, value_cache.shape[3],
-                attn_metadata.max_seq_len, alibi, self.kv_cache_dtype, layer._k_scale, layer._v_scale):
-            return output
-        else:
-            seq_lens, block_table = expand_to_token_sequences(
-                attn_metadata.query_start_loc, attn_metadata.seq_lens, attn_metadata.block_table, n)
-        out = PagedAttention.forward_decode(
-            q, key_cache, value_cache, block_table, seq_lens, attn_metadata.max_seq_len,
+        out = output[:n].view(n, self.num_heads, self.head_size)
+        seq_lens, block_table, starts = md.seq_lens, md.block_table, md.query_start_loc
+        first = 0  # row of the first request that is left
+        if cascade:
+            first = min(num_decodes, n)
+            PagedAttention.forward_decode_shared_prefix(
+                q[:first], key_cache, value_cache, block_table, seq_lens, md.common_prefix_len, md.max_seq_len,
+                self.kv_cache_dtype, self.num_kv_heads, self.scale, alibi, layer._k_scale, layer._v_scale,
+                output=out[:first])
+            if first == n:
+                return output
+            seq_lens, block_table, starts, num_decodes = seq_lens[first:], block_table[first:], starts[first:], 0
+        if md.max_query_len > 1:
+            # (rows of q and out go by `starts`, whatever is in front of the first request)
+            if ops.paged_attention_varlen(
+                    out, q, key_cache, value_cache, self.num_kv_heads, self.scale, block_table, seq_lens, starts,
+                    num_decodes, value_cache.shape[3], md.max_seq_len, alibi, self.kv_cache_dtype, layer._k_scale,
+                    layer._v_scale):
+                return output
+            seq_lens, block_table = expand_to_token_sequences(starts - first, seq_lens, block_table, n - first)
+        out[first:].copy_(PagedAttention.forward_decode(
+            q[first:], key_cache, value_cache, block_table, seq_lens, md.max_seq_len,
             self.kv_cache_dtype, self.num_kv_heads, self.scale, alibi, layer._k_scale,
-            layer._v_scale)
-        output[:n].view(n, self.num_heads, self.head_size).copy_(out)
+            layer._v_scale))
         return output
 
 
@@ -252,5 +281,13 @@ class B200PagedAttentionBackend:
                                                  cache_dtype_str)
 
     @staticmethod
-    def use_cascade_attention(*args, **kwargs) -> bool:
-        return False
+    def use_cascade_attention(common_prefix_len: int = 0, query_lens=None, num_query_heads: int = 0,
+                              num_kv_heads: int = 0, use_alibi: bool = False, use_sliding_window: bool = False,
+                              use_local_attention: bool = False, num_sms: int = 0, dcp_world_size: int = 1,
+                              **kwargs) -> bool:
+        """Whether a step with this common prefix is built as a cascade: there are decodes to share it
+        (``query_lens``: new tokens of the requests, the single ones in front).  Which kernels it runs on -
+        the ordinary ones where there is too little to share - is decided from the sizes of the batch."""
+        if common_prefix_len <= 0 or query_lens is None or use_sliding_window or use_local_attention:
+            return False
+        return dcp_world_size == 1 and len(query_lens) > 1 and int(query_lens[0]) == int(query_lens[1]) == 1

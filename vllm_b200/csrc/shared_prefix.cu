@@ -92,9 +92,9 @@ static int64_t unit_ns(int head_size, int row_tiles, int turns, int64_t tile_byt
 
 // Which way a call goes: 0 the ordinary kernels on whole sequences; behind the prefix the direct kernel (1), the same
 // with a warp to an item (2), or the persistent one beside the prefix and a third launch (3).  What each takes, us:
-// fitted to 260 random batches (2 to 2000 sequences, prefixes of 64 to 65000 tokens, up to 3000 own ones, all head sizes,
-// cache types and ten head counts; own lengths are taken as half the bound).  The choice is 3 % from the best of the four
-// on average, more than 25 % in 9 cases; each of them alone 82, 21, 85 and 50 %.
+// fitted to 410 random batches (2 to 2000 sequences, prefixes of 64 to 65000 tokens, up to 3000 own ones, all head sizes,
+// cache types and ten head counts; own lengths are taken as half the bound).  The choice is 2.3 % from the best of the
+// four on average, more than 25 % in 7 cases; each of them alone 81, 23, 87 and 52 %.
 //   prefix_all: the prefix's work over all SMs; prefix_cut: of its longest CTA
 static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const SharedPrefixPlan& r, double prefix_all,
                              double prefix_cut, bool tails) {
@@ -103,21 +103,22 @@ static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const Sh
   const double own = std::max(a.max_seq_len - prefix_len, 1), tiles = own / 16 + 0.5;
   const double row = a.num_kv_heads * D * 2 * es, hbm = N * own / 2 * row * us;
   const double latency = (es == 1 ? 0.63 + 0.0037 * D : 0.43 + 0.0061 * D) * (group > 8 ? 1.4 : 1);  // of a tile
-  const double prefix = 8 + prefix_cut, places = 3.0 * sms, warps = r.cluster * kDirectWarps, items = double(r.items);
+  const double prefix = 6.5 + prefix_cut, places = 3.0 * sms, warps = r.cluster * kDirectWarps, items = double(r.items);
   const double waves = std::max(1.0, items * r.cluster / places), solo_waves = std::max(1.0, items / places / kDirectWarps);
   // trips to the prefix's parts, of which a row of few sequences has over a hundred
   const double parts = (double(r.key_tiles) / r.cut + 1) * (r.turns ? 2 : 1);
   const double rounds = std::ceil(parts / (4 * r.cluster)) * std::ceil(std::min(group, 16) * D / 4 / 128);
   double t[4];
-  t[0] = 14.6 + 1.24 * N * (prefix_len + own / 2) * row * us;
-  t[1] = prefix + 6 + std::max({1.2 * hbm, 1.9 * tiles / warps * latency,
-                                waves * (2.6 + std::max(own / 32 / warps, 0.5) * latency)}) +
-         0.8 * std::max(rounds - 4, 0.0);
-  t[2] = prefix + 5 + std::max({1.2 * hbm, 0.9 * tiles * latency, solo_waves * (3.4 + std::max(own / 32, 1.0) * latency)}) +
-         0.8 * std::max(parts - 8, 0.0);
+  t[0] = 14.2 + std::max(N * (prefix_len + own / 2) * row * us, 1.13 * (prefix_len + own / 2) / 1024 * latency) +
+         (group > 8 && D > 128 ? 30 : 0);  // (two head tiles of a wide head: the persistent kernel only)
+  t[1] = prefix + 6 + std::max({2.9 * hbm, 0.75 * tiles / warps * latency,
+                                waves * (4 + 1.2 * std::max(own / 32 / warps, 0.5) * latency)}) +
+         0.43 * std::max(rounds - 4, 0.0);
+  t[2] = prefix + 5 + std::max({1.2 * hbm, 0.95 * tiles * latency, solo_waves * (5.6 + 0.8 * std::max(own / 32, 1.0) * latency)}) +
+         0.43 * std::max(parts - 8, 0.0);
   const double tail_items = N * a.num_kv_heads * ((group + (group <= 8 ? 7 : 15)) / (group <= 8 ? 8 : 16));
   const double beside = (N * own / 2 * row / 65e3 + tail_items * 0.5) / sms;
-  t[3] = tails ? 31 + std::max(prefix_all + beside, hbm) + 0.7e-6 * N * a.num_heads * D * 4 : 1e30;
+  t[3] = tails ? 30 + std::max(prefix_all + beside, hbm) + 0.6e-6 * N * a.num_heads * D * 4 : 1e30;
   return int(std::min_element(t, t + 4) - t);
 }
 

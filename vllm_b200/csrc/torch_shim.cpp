@@ -888,7 +888,9 @@ PyObject* py_rotary_flash(PyObject*, PyObject* const* a, Py_ssize_t n) { return 
 PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!plain_state()) Py_RETURN_FALSE;
   Args in{a, n};
-  at::Tensor out = in.tensor(), q = in.tensor(), k = in.tensor(), v = in.tensor(), cache = in.tensor();
+  at::Tensor out = in.tensor(), q = in.tensor();
+  const auto new_k = in.optional_tensor(), new_v = in.optional_tensor();  // (none: nothing to write)
+  at::Tensor cache = in.tensor();
   at::Tensor bt = in.tensor(), sl = in.tensor(), slots = in.tensor(), qsl = in.tensor();
   at::Tensor ks = in.tensor(), vs = in.tensor();
   const auto alibi = in.optional_tensor();
@@ -908,7 +910,9 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     };
     if (type != ScalarType::BFloat16 && type != ScalarType::Half) return false;
     if (tokens <= 0 || H <= 0 || HK <= 0 || D <= 0 || H % HK != 0) return false;
-    if (!rows(q, H) || !rows(k, HK) || !rows(v, HK)) return false;
+    if (write && (!new_k.has_value() || !new_v.has_value())) return false;
+    const at::Tensor k = new_k.value_or(q), v = new_v.value_or(q);
+    if (!rows(q, H) || (new_k.has_value() && !rows(k, HK)) || (new_v.has_value() && !rows(v, HK))) return false;
     if (!out.is_contiguous() || out.numel() < tokens * H * D || out.scalar_type() != type) return false;
     if (cache.dim() != 3 || cache.size(0) != 2 || !cache.is_contiguous() || cache.size(2) % (HK * D) != 0)
       return false;
@@ -929,7 +933,7 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       return false;
     }
     const auto dev = q.device();
-    for (const at::Tensor* t : {&out, &k, &v, &cache, &bt, &sl, &slots, &qsl, &ks, &vs})
+    for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&out, &k, &v, &cache, &bt, &sl, &slots, &qsl, &ks, &vs})
       if (t->device() != dev) return false;
 
     char* base = static_cast<char*>(cache.data_ptr());

@@ -42,6 +42,35 @@ class PagedAttention:
                               kv_cache_dtype, k_scale, v_scale)
 
     @staticmethod
+    def rotate_and_write_to_paged_cache(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor,
+                                        positions: torch.Tensor, cos_sin_cache: torch.Tensor, is_neox: bool,
+                                        key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                        slot_mapping: torch.Tensor, kv_cache_dtype: str, k_scale: torch.Tensor,
+                                        v_scale: torch.Tensor,
+                                        query_out: torch.Tensor | None = None) -> torch.Tensor:
+        """``write_to_paged_cache`` with queries and keys rotated by their positions on the way; returns
+        the rotated queries (`query_out`, which may be `query` itself; a new tensor by default)."""
+        if query_out is None:
+            query_out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        ops.rotary_reshape_and_cache(query_out, positions, query, key, value, cos_sin_cache, is_neox, key_cache,
+                                     value_cache, slot_mapping.flatten(), kv_cache_dtype, k_scale, v_scale)
+        return query_out
+
+    @staticmethod
+    def forward_decode_shared_prefix(query: torch.Tensor, key_cache: torch.Tensor, value_cache: torch.Tensor,
+                                     block_tables: torch.Tensor, seq_lens: torch.Tensor, prefix_len: int,
+                                     max_seq_len: int, kv_cache_dtype: str, num_kv_heads: int, scale: float,
+                                     alibi_slopes: torch.Tensor | None, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                                     output: torch.Tensor | None = None) -> torch.Tensor:
+        """``forward_decode`` for sequences that begin with the same `prefix_len` tokens, in the same blocks."""
+        if output is None:
+            output = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+        ops.paged_attention_shared_prefix(output, query, key_cache, value_cache, num_kv_heads, scale, block_tables,
+                                          seq_lens, prefix_len, value_cache.shape[3], max_seq_len, alibi_slopes,
+                                          kv_cache_dtype, k_scale, v_scale)
+        return output
+
+    @staticmethod
     def use_v1(max_seq_len: int, num_seqs: int, num_heads: int) -> bool:
         """The reference's choice between v1 and v2 (paged_attn.py:134-136)."""
         partitions = (max_seq_len + _PARTITION_SIZE - 1) // _PARTITION_SIZE
