@@ -142,14 +142,19 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // queries are most; a chain of trips to memory (position -> table, slot -> store) for decode steps.  Blocks of one
 // launch do different things:
 //   * Q, K and V of the flash layout: a thread owns one unit of a head (the two chunks that a rotation of halves
-//     combines, or one chunk) of one token, loads its cosines and sines once and walks over heads, four at a time;
+//     combines, or one chunk) of one token, loads its cosines and sines once and walks over heads, four chunks at a time;
 //   * V of the x-layout is a transpose: a warp takes 16 tokens x up to 64 dimensions of a head through shared
 //     memory (ldmatrix.trans gives a lane four tokens of a dimension).  Tiles are moved onto 16-slot boundaries of
 //     the cache as in the other KV write kernels (kv_write_windows.h).
+// Measured on B200: 8192 tokens of 32 / 8 heads of 128, bf16, 42 us (4.9 TB/s of the 206 MB that it has to move); 16384
+// of 64 / 8 heads to fp8, chunks that start anywhere, 123 (5.2 TB/s; 139 with 24 warps to an SM and eight chunks a
+// thread, 24 and six 129, 16 and sixteen 141, 32 and eight, which spill, 152); flash layout, neighbours, a quarter
+// rotated, to e5m2, 51 (4.9; 61).  The next heads' chunks on their way under the ones in work need registers that are
+// not there (spills: 47 -> 57).  What is left is latency: a warp loads, waits, turns and stores.
 template <typename in_t, int KV, bool kHalves>
-__global__ void __launch_bounds__(kRotaryThreads, 3) rotary_write_kernel(const RotaryParams p, const RotaryPlan plan) {
+__global__ void __launch_bounds__(kRotaryThreads, 4) rotary_write_kernel(const RotaryParams p, const RotaryPlan plan) {
   using cache_t = std::conditional_t<KV == kKvAuto, in_t, uint8_t>;
-  constexpr int E = sizeof(cache_t), HU = 4;
+  constexpr int E = sizeof(cache_t), HU = kHalves ? 2 : 4;
   __shared__ __align__(16) unsigned char s_tile[kRotaryThreads / 32][16 * kRotaryPitch];
   const int tid = threadIdx.x;
   const int D = p.head_size, HK = p.num_kv_heads, B = p.block_size, N = p.num_tokens;
@@ -411,9 +416,9 @@ static bool rotary_plan(const RotaryParams& p, int cache_size, RotaryPlan* plan)
   while (r.tokens * 2 <= rows && r.tokens < N) r.tokens *= 2;
   r.lanes = rows / r.tokens;
   const int64_t tiles = (int64_t(N) + r.tokens - 1) / r.tokens;
-  // heads of a block: 8 to a thread, fewer while that leaves SMs without blocks
+  // heads of a block: 8 to a thread (16 where a unit is one chunk), fewer while that leaves SMs without blocks
   auto divide = [&](int heads, int& per, int& parts) -> int64_t {
-    per = std::min(heads, 8 * r.lanes);
+    per = std::min(heads, (p.neighbours ? 16 : 8) * r.lanes);
     while (per > r.lanes && tiles * ((heads + per - 1) / per) < 4 * sms) per = std::max(r.lanes, per / 2);
     parts = (heads + per - 1) / per;
     return tiles * parts;
