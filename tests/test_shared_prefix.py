@@ -381,6 +381,7 @@ def _route(prefix=256, **kw):
 def test_which_way_a_call_goes():
     """Little to share: the ordinary kernels.  Few sequences with short own parts, many with short ones, long ones."""
     assert _route(num_seqs=1) == 0 and _route(prefix=0) == 0 and _route(num_seqs=4, prefix=64) == 0
+    assert capi.shared_prefix_scratch_bytes(_c_args(num_seqs=4)[0], 64) == 0
     assert _route(num_seqs=64, prefix=4096, max_seq_len=4096 + 60) == 1
     assert _route(num_seqs=2000, num_heads=64, num_kv_heads=8, prefix=4096, max_seq_len=4096 + 100) == 2
     assert _route(num_seqs=256, num_heads=32, num_kv_heads=8, prefix=4096, max_seq_len=4096 + 1000) == 3

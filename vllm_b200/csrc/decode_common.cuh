@@ -112,11 +112,11 @@ struct SharedPrefixParts {
   template <int D>
   __device__ __forceinline__ Row row(int seq, int kvh, int head, int group) const {
     constexpr int64_t kPart = 128 * (D * 4 + 8);
-    const int tile = seq / tokens, grp = turns ? tile : tile / tiles;
-    const int64_t it = int64_t(kvh) * groups + grp, u0 = it * key_tiles;
-    const int c0 = int(u0 / cut), c1 = int((u0 + key_tiles - 1) / cut);
-    return {parts + ((it + c0) * tiles + (turns ? 0 : tile - grp * tiles)) * kPart, turns ? kPart : tiles * kPart,
-            (c1 - c0 + 1) * (turns ? 2 : 1), (seq - tile * tokens) * group + head};
+    const unsigned tile = unsigned(seq) / unsigned(tokens), grp = turns ? tile : tile / unsigned(tiles);
+    const unsigned it = unsigned(kvh) * unsigned(groups) + grp, u0 = it * unsigned(key_tiles);  // (below 2^30)
+    const int c0 = int(u0 / unsigned(cut)), c1 = int((u0 + key_tiles - 1) / unsigned(cut));
+    return {parts + (int64_t(it + c0) * tiles + (turns ? 0 : tile - grp * tiles)) * kPart, turns ? kPart : tiles * kPart,
+            (c1 - c0 + 1) * (turns ? 2 : 1), (seq - int(tile) * tokens) * group + head};
   }
 };
 

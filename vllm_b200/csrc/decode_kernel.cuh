@@ -907,7 +907,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
   while (inflight < NSLOT && produce_one()) {}
 
   // fold the per-tensor scales of an fp8 cache into the logit scale and the output scale
-  const float kv_qk = kFp8 ? *p.k_scale : 1.f;
+  const float kv_qk = kFp8 ? (kBehind ? __ldcg(p.k_scale) : *p.k_scale) : 1.f;
   const float kv_o = kFp8 ? *p.v_scale : 1.f;
   const float qk_scale = p.scale * kLog2e * kv_qk;
   bool failed = false;
@@ -953,7 +953,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int hl = nt * 8 + 2 * c + j;
-        slope[nt][j] = (has_alibi && hl < nheads) ? p.alibi[hq0 + hl] * kLog2e : 0.f;
+        slope[nt][j] = (has_alibi && hl < nheads) ? (kBehind ? __ldcg(p.alibi + hq0 + hl) : p.alibi[hq0 + hl]) * kLog2e : 0.f;
       }
 
     float o[KS][GP][4];

@@ -35,7 +35,7 @@ struct Tuning {
   int direct = 0;        // B200PA_TUNE_DIRECT: 1 always the direct kernel where it is built, 2 never
   int cluster = 0;       // B200PA_TUNE_CLUSTER: its CTAs per cluster
   int behind = 0;        // B200PA_TUNE_BEHIND: 1 direct, 2 solo, 3 persistent kernel behind a shared prefix
-  int prefix = 0;        // B200PA_TUNE_PREFIX: most CTAs of a shared prefix's kernel
+  int prefix = 0;        // B200PA_TUNE_PREFIX: a shared prefix's work in percent of the estimate
   int reload = 0;
 };
 Tuning tuning();

@@ -85,8 +85,10 @@ static SharedPrefixKernels find_shared_prefix(const b200pa_attn_args& a) {
 // What the prefix's kernel takes for a key tile of an item, ns of an SM: two row tiles in turns on the tensor cores, or
 // one by itself (measured: 128 fp8 sequences, 64 / 8 heads of 128, behind 8192 2.3 us; 8 sequences behind 65008 1.55;
 // head sizes 64 and 256 2.0 and 1.8), or its K and V on the way.
-static int64_t unit_ns(int head_size, int row_tiles, int turns, int64_t tile_bytes) {
-  const int64_t work = row_tiles == 1 ? 1800 : turns ? 1000 + 4 * head_size : 1500 + 8 * std::min(head_size, 128);
+static int64_t unit_ns(int head_size, int row_tiles, int turns, bool biased, bool fp8, int64_t tile_bytes) {
+  int64_t work = row_tiles == 1 ? 1800 : turns ? 1000 + 4 * head_size : 1500 + 8 * std::min(head_size, 128);
+  if (biased) work = work * 3 / 2;
+  else if (fp8 && !turns) work = work * 17 / 20;
   return std::max(work, tile_bytes * 1000 / 60000);
 }
 
@@ -141,25 +143,25 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   r.grid = int((units + r.cut - 1) / r.cut);
   const int es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1;
   auto up = [](int64_t v) { return (v + 255) & ~int64_t(255); };
-  r.own_at = up((items + r.grid) * r.tiles * int64_t(k.part_bytes));
-  r.bytes = r.own_at;
 
   // ---- behind the prefix
   const int gp = group <= 8 ? 1 : 2, heads = 8 * gp;
   const int64_t tail_items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + heads - 1) / heads);
   r.items = int64_t(a.num_seqs) * a.num_kv_heads * ((group + k.heads - 1) / k.heads);
-  if (r.items > INT32_MAX / 16) return r;
-  const int64_t unit = unit_ns(a.head_size, k.row_tiles, r.turns, int64_t(k.keys) * a.head_size * 2 * es);
+  if (r.items > INT32_MAX / 16) return {};
+  const int64_t unit = unit_ns(a.head_size, k.row_tiles, r.turns, a.alibi_slopes != nullptr, es == 1,
+                               int64_t(k.keys) * a.head_size * 2 * es);
   const int64_t places = int64_t(sms) * k.ctas_per_sm;
   const int64_t own_tiles = (int64_t(std::max(a.max_seq_len - prefix_len, 1)) + 15) / 16;
   // CTAs of a sequence and head: as many as the GPU takes at once, but no more warps than there are 16-token tiles
   while (r.cluster < 8 && r.items * r.cluster * 10 <= places * 6 && r.cluster * kDirectWarps < own_tiles) r.cluster *= 2;
   if (tune.cluster) r.cluster = tune.cluster;
-  const bool tails = tail_items <= INT32_MAX / 16 && plan_tails(a, gp, r);
+  const bool tails = tail_items <= INT32_MAX / 16 && sms >= 16 && plan_tails(a, gp, r);
   const int way = tune.behind ? tune.behind : shared_prefix_way(a, prefix_len, r, units * unit * 1e-3 / sms, r.cut * unit * 1e-3, tails);
-  if (way == 0) return r;
+  if (way == 0) return {};
   if (way != 3) r.tails.fn = nullptr;
   if (way == 2) r.cluster = 0;
+  r.bytes = up((items + r.grid) * r.tiles * int64_t(k.part_bytes));
   if (r.tails.fn != nullptr) {
     r.items = tail_items;
     r.heads = heads;
@@ -332,6 +334,7 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
   c.group = p.group;
   c.head_groups = d.head_groups;
   c.heads = plan.heads;
+  c.ranges = sm_count() * plan.warps;
   // threads that share four dimensions of a head: 1, 2, 4 ... 32, so that each adds up a few parts
   const int64_t most = int64_t(plan.key_tiles) * p.num_kv_heads * plan.groups < sm_count() ? plan.key_tiles
                        : sm_count() / (p.num_kv_heads * plan.groups) + 2;

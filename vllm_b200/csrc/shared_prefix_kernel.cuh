@@ -706,6 +706,7 @@ struct CombineParams {
   SharedPrefixParts pre;
   int num_seqs, num_heads, group, head_groups, heads, D;  // heads: of an item
   int share;                                              // threads to a unit
+  int ranges;                                             // most that the persistent kernel can have had
 };
 
 template <typename QT>
@@ -719,7 +720,10 @@ __global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(
   const int kvh = sub / p.head_groups, hg = sub - kvh * p.head_groups;
   const int nheads = min(HPI, p.group - hg * HPI), units = nheads * (D / 4);
   const int cut = __ldcg(p.cut);
-  const int2 found = __ldcg(p.pre.found + blockIdx.x);
+  int2 found = __ldcg(p.pre.found + blockIdx.x);
+  // (in bounds whatever is there: a wait of the launch in front that ran out leaves items out)
+  found.x = min(max(found.x, 0), p.ranges - 1);
+  found.y = min(max(found.y, 0), p.ranges - found.x);
   const int64_t own_slot = int64_t(HPI) * (D * 4 + 8), part = 128 * (D * 4 + 8);
   const unsigned char* own = p.pre.own + (int64_t(blockIdx.x) + found.x) * own_slot;
   // (SharedPrefixParts::row, with the cut that the prefix's kernel has chosen)

@@ -250,6 +250,9 @@ void paged_attention_shared_prefix(torch::Tensor& out, torch::Tensor& query, tor
   const auto dev = query.device();
   for (const torch::Tensor* t : {&out, &key_cache, &value_cache, &block_tables, &seq_lens})
     TORCH_CHECK(t->device() == dev, "all tensors must be on one device");
+  TORCH_CHECK((a.kv_dtype == B200PA_KV_AUTO || (k_scale.device() == dev && v_scale.device() == dev)) &&
+                  (!alibi_slopes.has_value() || alibi_slopes->device() == dev),
+              "all tensors must be on one device");
   if (lse.has_value()) {
     TORCH_CHECK(lse->device() == dev && lse->scalar_type() == at::ScalarType::Float && lse->is_contiguous() &&
                     lse->dim() == 2 && lse->size(0) == query.size(1) && lse->size(1) == n,
@@ -394,6 +397,8 @@ void rotary_write(torch::Tensor& query_out, torch::Tensor& positions, torch::Ten
               "the caches do not have the key's heads and head size");
   for (const torch::Tensor* t : {&query_out, &positions, &query, &value, &cos_sin_cache, &key_cache, &value_cache, &slot_mapping})
     TORCH_CHECK(t->device() == key.device(), "all tensors must be on one device");
+  TORCH_CHECK(a.kv_dtype == B200PA_KV_AUTO || (k_scale.device() == key.device() && v_scale.device() == key.device()),
+              "all tensors must be on one device");
   b200pa_rotary_args r;
   std::memset(&r, 0, sizeof(r));
   r.query_out = query_out.data_ptr();
