@@ -648,9 +648,12 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
   __syncthreads();
 
   const unsigned ctas = kBehind ? unsigned(s_plan[3]) : gridDim.x;
-  if (kBehind && blockIdx.x >= ctas) {
-    grid_dependency();
-    return;
+  if constexpr (kBehind) {
+    grid_launch_dependents();  // (the launch that adds up starts with its wait for this one)
+    if (blockIdx.x >= ctas) {
+      grid_dependency_wait();
+      return;
+    }
   }
   const unsigned grid_warps = ctas * unsigned(nwarps);
   // work items of an unsplit launch / ranges of a split one
@@ -1441,7 +1444,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
   }
 
   if constexpr (kBehind) {
-    grid_dependency();  // (so that this grid's end is the prefix's as well)
+    grid_dependency_wait();  // (so that this grid's end is the prefix's as well)
     return;
   }
   // ---- last CTA out re-arms the scheduler words for the next launch

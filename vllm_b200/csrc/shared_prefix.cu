@@ -120,7 +120,7 @@ static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const Sh
          0.43 * std::max(parts - 8, 0.0);
   const double tail_items = N * a.num_kv_heads * ((group + (group <= 8 ? 7 : 15)) / (group <= 8 ? 8 : 16));
   const double beside = (N * own / 2 * row / 65e3 + tail_items * 0.5) / sms;
-  t[3] = tails ? 30 + std::max(prefix_all + beside, hbm) + 0.6e-6 * N * a.num_heads * D * 4 : 1e30;
+  t[3] = tails ? 25 + std::max(prefix_all + beside, hbm) + 0.6e-6 * N * a.num_heads * D * 4 : 1e30;
   return int(std::min_element(t, t + 4) - t);
 }
 
@@ -340,10 +340,11 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
                        : sm_count() / (p.num_kv_heads * plan.groups) + 2;
   c.share = 1;
   while (c.share < 32 && c.share * 6 < most * (plan.turns ? 2 : 1)) c.share *= 2;
-  const int lanes = kCombineThreads / c.share, per_item = std::min(p.group, plan.heads) * (a->head_size / 4);
   c.D = a->head_size;
+  const int per_item = std::min(p.group, plan.heads) * (a->head_size / 4);
+  const int threads = std::min(kCombineThreads, (per_item * c.share + 31) / 32 * 32), lanes = threads / c.share;
   e = launch_dependent(a->q_dtype == B200PA_BF16 ? shared_prefix_combine_kernel<__nv_bfloat16> : shared_prefix_combine_kernel<__half>,
-                       dim3(unsigned(plan.items), unsigned((per_item + lanes - 1) / lanes)), dim3(kCombineThreads), 0, s, c);
+                       dim3(unsigned(plan.items), unsigned((per_item + lanes - 1) / lanes)), dim3(threads), 0, s, c);
   count_launch();
   if (e != cudaSuccess) {
     set_error("shared prefix combine kernel launch failed: %s", cudaGetErrorString(e));

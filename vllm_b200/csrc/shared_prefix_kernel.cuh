@@ -714,36 +714,36 @@ __global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(
   constexpr bool kBf = std::is_same_v<QT, __nv_bfloat16>;
   __shared__ float4 s_acc[kCombineThreads];
   __shared__ float2 s_ml[kCombineThreads];
+  const unsigned tid = threadIdx.x, D = p.D, HPI = p.heads, item = blockIdx.x;
+  const unsigned sub = item / unsigned(p.num_seqs), seq = item - sub * unsigned(p.num_seqs);
+  const unsigned kvh = sub / unsigned(p.head_groups), hg = sub - kvh * unsigned(p.head_groups);
+  const unsigned nheads = min(HPI, p.group - hg * HPI), units = nheads * (D / 4);
+  const unsigned share = p.share, lanes = blockDim.x / share;
+  const unsigned z = tid / lanes, u = blockIdx.y * lanes + tid - z * lanes;
+  const bool on = u < units;
+  const unsigned d4 = on ? u / nheads : 0, hl = on ? u - d4 * nheads : 0;
+  // (SharedPrefixParts::row, with the cut that the prefix's kernel has chosen)
+  const unsigned tile = seq / unsigned(p.pre.tokens), grp = p.pre.turns ? tile : tile / unsigned(p.pre.tiles);
+  const unsigned it = kvh * unsigned(p.pre.groups) + grp, u0 = it * unsigned(p.pre.key_tiles);
+  const int row = int(seq - tile * p.pre.tokens) * p.group + hg * HPI;
+  const int64_t own_slot = int64_t(HPI) * (D * 4 + 8), part = 128 * (D * 4 + 8);
   grid_dependency();
-  const int tid = threadIdx.x, D = p.D, HPI = p.heads;
-  const int seq = blockIdx.x % p.num_seqs, sub = blockIdx.x / p.num_seqs;
-  const int kvh = sub / p.head_groups, hg = sub - kvh * p.head_groups;
-  const int nheads = min(HPI, p.group - hg * HPI), units = nheads * (D / 4);
-  const int cut = __ldcg(p.cut);
-  int2 found = __ldcg(p.pre.found + blockIdx.x);
+  const unsigned cut = __ldcg(p.cut);
+  int2 found = __ldcg(p.pre.found + item);
+  const float v_scale = p.v_scale ? __ldcg(p.v_scale) : 1.f;
   // (in bounds whatever is there: a wait of the launch in front that ran out leaves items out)
   found.x = min(max(found.x, 0), p.ranges - 1);
   found.y = min(max(found.y, 0), p.ranges - found.x);
-  const int64_t own_slot = int64_t(HPI) * (D * 4 + 8), part = 128 * (D * 4 + 8);
-  const unsigned char* own = p.pre.own + (int64_t(blockIdx.x) + found.x) * own_slot;
-  // (SharedPrefixParts::row, with the cut that the prefix's kernel has chosen)
-  const int tile = seq / p.pre.tokens, grp = p.pre.turns ? tile : tile / p.pre.tiles;
-  const int64_t it = int64_t(kvh) * p.pre.groups + grp, u0 = it * p.pre.key_tiles;
-  const int c0 = int(u0 / cut), c1 = int((u0 + p.pre.key_tiles - 1) / cut);
+  const unsigned char* own = p.pre.own + (int64_t(item) + found.x) * own_slot;
+  const unsigned c0 = u0 / cut, c1 = (u0 + p.pre.key_tiles - 1) / cut;
   const unsigned char* first =
-      p.pre.parts + ((it + c0) * p.pre.tiles + (p.pre.turns ? 0 : tile - grp * p.pre.tiles)) * part;
+      p.pre.parts + (int64_t(it + c0) * p.pre.tiles + (p.pre.turns ? 0 : tile - grp * p.pre.tiles)) * part;
   const int64_t step = p.pre.turns ? part : p.pre.tiles * part;
-  const int row = (seq - tile * p.pre.tokens) * p.group + hg * HPI;
-  const int np = found.y, n = np + (c1 - c0 + 1) * (p.pre.turns ? 2 : 1);
-  const float v_scale = p.v_scale ? __ldcg(p.v_scale) : 1.f;
+  const int np = found.y, n = np + int(c1 - c0 + 1) * (p.pre.turns ? 2 : 1);
 
-  const int share = p.share, lanes = kCombineThreads / share;
-  const int u = blockIdx.y * lanes + tid % lanes, z = tid / lanes;
-  const bool on = u < units;
-  const int hl = on ? u % nheads : 0, d4 = on ? u / nheads : 0;
   float m = -INFINITY, l = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int k0 = z; k0 < n && on; k0 += 4 * share) {
+  for (int k0 = int(z); k0 < n && on; k0 += 4 * share) {
     float2 ml[4];
     float4 v[4];
 #pragma unroll
@@ -779,7 +779,7 @@ __global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(
     s_ml[tid] = make_float2(m, l);
     __syncthreads();
     if (z > 0 || !on) return;
-    for (int k = 1; k < share; ++k) {
+    for (unsigned k = 1; k < share; ++k) {
       const float2 ml = s_ml[tid + k * lanes];
       if (ml.y == 0.f) continue;
       const float4 v = s_acc[tid + k * lanes];
