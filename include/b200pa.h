@@ -232,7 +232,7 @@ int b200pa_paged_attention_varlen_supported(const b200pa_attn_args* args);
  * prefix is read through row 0, or through every row where the call runs as paged_attention_v1.)  No counterpart in
  * the reference's paged-attention ops.
  *   args: as for v1 (out_lse included; seq_lens, max_seq_len and the block tables cover prefix and own tokens);
- *     block-sparse arguments are not supported.  A sequence shorter than the prefix sees the keys that it has.
+ *     block-sparse arguments are not supported.  A sequence shorter than the prefix attends to the tokens that it has.
  *   prefix_len: a multiple of block_size, 0 included
  *   scratch: device memory on a 16-byte boundary, of b200pa_shared_prefix_scratch_bytes bytes at least; its
  *     contents do not matter, and nothing else is kept between calls: calls with scratch of their own may overlap

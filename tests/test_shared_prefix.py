@@ -166,6 +166,24 @@ def test_sequences_without_own_tokens_and_shorter_ones(N):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv,behind", [("auto", 6), ("fp8_e5m2", 6), ("auto", 300), ("fp8_e5m2", 300)])
+def test_prefix_values_that_a_shorter_sequence_does_not_see(kv, behind):
+    """An infinite value of the prefix reaches the sequences that have it, and no other one."""
+    c = Case(own=(-100, behind, -255, -1, behind, -256) * 15, prefix=256, kv=kv)
+    c.vc[c.bt[0, 15], :, 5, 15] = 0x7C if kv != "auto" else float("inf")  # the prefix's last token
+    lse = torch.full((c.H, c.N), 5.0, device=DEV)
+    got = c.call(lse=lse)
+    full = c.lens >= c.prefix
+    assert (got[full][:, :, 5] == float("inf")).all()
+    out, mag, want_lse = c.want()
+    u = torch.finfo(torch.float16 if kv != "auto" else c.dtype).eps / 2
+    tol = mag * (u + 2.0 ** -16) + out.abs() * 2.0 ** -8 + 2.0 ** -22
+    short = (~full).nonzero().flatten()
+    assert ((got[short].double() - out[short]).abs() <= tol[short]).all()
+    assert ((lse.double() - want_lse).abs()[:, c.lens > 0] <= 1e-5 * (1 + want_lse.abs()[:, c.lens > 0])).all()
+
+
+@pytest.mark.gpu
 def test_all_rows_empty_or_no_sequences():
     c = Case(own=(-256, -256, -300), prefix=256)
     assert (c.call() == 0).all()

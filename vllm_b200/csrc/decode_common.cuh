@@ -86,6 +86,13 @@ __device__ __forceinline__ int work_units(int len, int block_size) {
   return max(2, ((len + block_size - 1) / block_size + 1) & ~1);
 }
 
+// Tokens that the launch behind a shared prefix has of a sequence of `len`: those behind the prefix; all of one that is
+// shorter, which takes nothing from the prefix's kernel (its weights of zero would meet whatever values the
+// others have there), and begins that many blocks earlier in the block table.
+__device__ __forceinline__ int behind_prefix(int len, int prefix_len) {
+  return len >= prefix_len ? len - prefix_len : max(len, 0);
+}
+
 // What the launch in front has of a prefix that all sequences share (shared_prefix_kernel.cuh): which part of
 // it covers what, for the kernels that have the sequences' own tokens and add the prefix to them.
 struct SharedPrefixParts {

@@ -90,8 +90,10 @@ struct DirectShape {
 };
 
 // grid.x = (sequence, kv head, head group) items x cluster size.  kBehind: attends to what a sequence has behind the
-// shared prefix, and adds the prefix's parts.  kSolo (many short sequences): every warp has an item of its own, nothing
-// is merged between warps; `cluster` is the number of items then.
+// shared prefix, and adds the prefix's parts, which the CTAs of a cluster share out (8 sequences have 38 parts each behind
+// 65008 tokens: 34 -> 20 us behind the prefix).  kSolo (many short sequences): every warp has an item of its own, nothing
+// is merged between warps; `cluster` is the number of items then (2000 sequences of 8 to 250 own tokens, 64 / 8 heads of
+// 128, fp8: 298 -> 134 us; it is bound by its dependent instructions, 0.41 of issue slots and 0.59 of HBM's rate).
 template <typename QT, int KV, int D, int GP, bool kBehind, bool kSolo = false>
 __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int cluster, const SharedPrefixParts& pre) {
   using TR = DecodeTraits<QT, KV, D, GP>;
@@ -127,7 +129,8 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
   // (kBehind: the prefix's kernel lets this one in when all before it is complete, and writes nothing but its parts)
   if (!kBehind && !p.early) grid_dependency();
 
-  const int len = kBehind ? max(__ldcg(p.seq_lens + seq) - pre.prefix_len, 0) : min(max(__ldcg(p.seq_lens + seq), 0), p.len_cap);
+  const int seq_len = kBehind ? __ldcg(p.seq_lens + seq) : 0;
+  const int len = kBehind ? behind_prefix(seq_len, pre.prefix_len) : min(max(__ldcg(p.seq_lens + seq), 0), p.len_cap);
   // ---- Q (B operand; n = head g): 16 bytes of K's chunk order per chunk of this lane
   uint32_t qf[GP][NI][SPC][2];
 #pragma unroll
@@ -173,7 +176,8 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
   const int tiles = (len + 15) >> 4;
   const int nw = kSolo ? 1 : cluster * kDirectWarps, gw = kSolo ? 0 : rank * kDirectWarps + warp;
   const int t_begin = int(int64_t(tiles) * gw / nw), t_end = int(int64_t(tiles) * (gw + 1) / nw);
-  const int* bt = p.block_tables + int64_t(seq) * p.max_blocks_per_seq;
+  const int* bt = p.block_tables + int64_t(seq) * p.max_blocks_per_seq -
+                  (kBehind && seq_len < pre.prefix_len ? pre.prefix_len >> b_shift : 0);
   const char* kb = static_cast<const char*>(p.kc) + int64_t(kvh) * p.kv_head_stride * ES;
   const char* vb = static_cast<const char*>(p.vc) + int64_t(kvh) * p.kv_head_stride * ES;
   const int64_t bstride = p.kv_block_stride * ES;

@@ -62,6 +62,7 @@ struct WorkItem {
   int tok_begin;
   int tok_end;
   int first_page;
+  int table_page;  // (behind a shared prefix) of the block table
   int npages;
   int win;         // which 32-page window `bt` holds
   int bt;          // per-lane block id of page first_page + 32*win + lane
@@ -82,7 +83,7 @@ template <bool kPastL1 = false>
 __device__ __forceinline__ int load_bt(const DecodeParams& p, const WorkItem& it, int win, int lane) {
   const int pg = win * 32 + lane;
   if (pg >= it.npages) return 0;
-  if constexpr (kPastL1) return __ldcg(p.block_tables + int64_t(it.seq) * p.max_blocks_per_seq + it.first_page + pg);
+  if constexpr (kPastL1) return __ldcg(p.block_tables + int64_t(it.seq) * p.max_blocks_per_seq + it.table_page + pg);
   return __ldg(p.block_tables + int64_t(it.seq) * p.max_blocks_per_seq + it.first_page + pg);
 }
 
@@ -587,7 +588,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     const int s0 = min(S, int(threadIdx.x) * per);
     const int s1 = min(S, s0 + per);
     auto units_of = [&](int s) {
-      const int len = kBehind ? max(__ldcg(p.seq_lens + s) - pre.prefix_len, 0) : min(max(__ldcg(p.seq_lens + s), 0), p.len_cap);
+      const int len = kBehind ? behind_prefix(__ldcg(p.seq_lens + s), pre.prefix_len) : min(max(__ldcg(p.seq_lens + s), 0), p.len_cap);
       return work_units(len, B);
     };
     int mine = 0, mx = 0;
@@ -734,6 +735,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     WorkItem it;
     it.valid = false;
     it.seq = it.kvh = it.hg = it.part = it.tok_begin = it.tok_end = it.first_page = it.npages = 0;
+    if constexpr (kBehind) it.table_page = 0;
     it.nparts = 1;
     it.win = 0;
     it.bt = 0;
@@ -766,7 +768,8 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     const int c0 = cum[st.z];
     const int n = cum[st.z + 1] - c0;      // units of this sequence
     const int take = min(n - st.y, st.x);  // units of it that fall into the range
-    const int len = kBehind ? max(__ldcg(p.seq_lens + st.z) - pre.prefix_len, 0) : min(max(p.seq_lens[st.z], 0), p.len_cap);
+    const int seq_len = kBehind ? __ldcg(p.seq_lens + st.z) : 0;
+    const int len = kBehind ? behind_prefix(seq_len, pre.prefix_len) : min(max(p.seq_lens[st.z], 0), p.len_cap);
     it.seq = st.z;
     it.kvh = st.w / p.head_groups;
     it.hg = st.w % p.head_groups;
@@ -783,6 +786,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
       it.part = int((base + st.y) / C) - w_lo;
     }
     it.first_page = st.y;
+    if constexpr (kBehind) it.table_page = st.y - (seq_len < pre.prefix_len ? pre.prefix_len / B : 0);
     it.tok_begin = st.y * B;
     it.tok_end = max(it.tok_begin, min(len, (st.y + take) * B));
     it.npages = (it.tok_end - it.tok_begin + B - 1) / B;
@@ -919,7 +923,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
   while (cur.valid && !failed) {
     const int hq0 = cur.kvh * p.group + cur.hg * TR::kHeadsPerItem;
     const int nheads = min(TR::kHeadsPerItem, p.group - cur.hg * TR::kHeadsPerItem);
-    const int seq_len = kBehind ? (has_alibi ? __ldcg(p.seq_lens + cur.seq) - pre.prefix_len : 0) : p.seq_lens[cur.seq];
+    const int seq_len = kBehind ? (has_alibi ? behind_prefix(__ldcg(p.seq_lens + cur.seq), pre.prefix_len) : 0) : p.seq_lens[cur.seq];
 
     // ---- Q fragments (B operand), head = nt*8 + g
     uint32_t qf[GP][KS][2];
@@ -1148,8 +1152,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
         unsigned char* vpage = my_slots + size_t(cons_slot) * slot_bytes +
                                (split_kv ? 0u : step_bytes) + pl * page_bytes;
         if constexpr (kBehind) {
-          // the 16 tokens of the last tile that is multiplied, 16 bytes at a time.  (Short sequences are masked
-          // often: 2000 of 8 to 250 tokens, 64 / 8 heads, fp8, 185 us with the loop below.)
+          // the 16 tokens of the last tile that is multiplied, 16 bytes at a time (short sequences are masked often)
           const int left = r & 15;  // valid tokens of the tile (0: all)
           if (left != 0) {
             for (int d = lane; d < D; d += 32) {

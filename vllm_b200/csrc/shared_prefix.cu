@@ -96,7 +96,7 @@ static int64_t unit_ns(int head_size, int row_tiles, int turns, bool biased, boo
 // with a warp to an item (2), or the persistent one beside the prefix and a third launch (3).  What each takes, us:
 // fitted to 410 random batches (2 to 2000 sequences, prefixes of 64 to 65000 tokens, up to 3000 own ones, all head sizes,
 // cache types and ten head counts; own lengths are taken as half the bound).  The choice is 2.3 % from the best of the
-// four on average, more than 25 % in 7 cases; each of them alone 81, 23, 87 and 52 %.
+// four on average, more than 25 % in 7 cases (on 150 others 3.6 %, in 6); each of them alone 81, 23, 87 and 52 %.
 //   prefix_all: the prefix's work over all SMs; prefix_cut: of its longest CTA
 static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const SharedPrefixPlan& r, double prefix_all,
                              double prefix_cut, bool tails) {
