@@ -149,7 +149,7 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 // Measured on B200: 8192 tokens of 32 / 8 heads of 128, bf16, 42 us (4.9 TB/s of the 206 MB that it has to move); 16384
 // of 64 / 8 heads to fp8, chunks that start anywhere, 123 (5.2 TB/s; 139 with 24 warps to an SM and eight chunks a
 // thread, 24 and six 129, 16 and sixteen 141, 32 and eight, which spill, 152); flash layout, neighbours, a quarter
-// rotated, to e5m2, 51 (4.9; 61).  The next heads' chunks on their way under the ones in work need registers that are
+// rotated, to e5m2, 47 (5.3).  The next heads' chunks on their way under the ones in work need registers that are
 // not there (spills: 47 -> 57).  What is left is latency: a warp loads, waits, turns and stores.
 template <typename in_t, int KV, bool kHalves>
 __global__ void __launch_bounds__(kRotaryThreads, 4) rotary_write_kernel(const RotaryParams p, const RotaryPlan plan) {
