@@ -225,6 +225,23 @@ def test_infinite_and_nan_keys_stay_with_their_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("H,HK", [(28, 4), (12, 4), (40, 8)])
+@pytest.mark.parametrize("dtype,kv", [("bf16", "auto"), ("fp16", "fp8"), ("bf16", "fp8_e5m2")])
+def test_rows_of_a_tile_without_a_sequence_change_nothing(H, HK, dtype, kv):
+    """Head groups that do not divide 128 leave rows of a tile unused: what the launch before has left in shared memory
+    there decides nothing, not even when the others are scaled again (the results are the same to the last bit)."""
+    c = Case(own=tuple(7 + 11 * i % 110 for i in range(200)), prefix=1504, H=H, HK=HK, dtype=dtype, kv=kv)
+    before = Case(own=(1,) * 64, prefix=8192, H=64, HK=8, dtype=dtype, kv=kv)  # (8 heads: every row in use, every SM)
+    q, got = before.q.clone(), []
+    for size in (0.0, 30.0):
+        before.q.copy_(q * size)
+        before.call()
+        got.append(c.call())
+    assert torch.equal(*got)
+    c.check(got[0])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kw", [dict(dtype="fp32"), dict(B=8), dict(own=(40,))])
 def test_shapes_without_a_kernel_run_as_ordinary_decodes(kw):
     c = Case(prefix=64, **kw)

@@ -256,7 +256,8 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
               for (int k = 0; k < 32; k += 2) h4[k / 2 & 3] = fmax3(h4[k / 2 & 3], x[ch][k], x[ch][k + 1]);
             const float mx = fmax3(fmaxf(h4[0], h4[1]), h4[2], h4[3]) * cc;
             // raise the maximum, and rescale what has been summed
-            const bool grow = mx > m + (kFp8 || biased ? 8.f : 0.f) || (m == -INFINITY && mx > m);
+            // (a row without a sequence decides nothing: where its query would be, shared memory holds anything)
+            const bool grow = valid && (mx > m + (kFp8 || biased ? 8.f : 0.f) || (m == -INFINITY && mx > m));
             if (__any_sync(0xffffffffu, grow)) {
               const float m_new = fmaxf(m, mx);
               const float alpha = m_new == -INFINITY ? 1.f : fast_exp2(m - m_new);
@@ -288,7 +289,7 @@ pa_shared_prefix_kernel(const SharedPrefixParams p, const __grid_constant__ CUte
               if (!kFp8) m4[k / 2 & 3] = fmax3(m4[k / 2 & 3], x[NC / 2 + ch][k], x[NC / 2 + ch][k + 1]);
             }
           const float mx = fmax3(fmaxf(m4[0], m4[1]), m4[2], m4[3]) * cc;
-          const bool low = (sa.x + sa.y) + (sb.x + sb.y) > 4096.f || mx > m + 12.f;
+          const bool low = valid && ((sa.x + sa.y) + (sb.x + sb.y) > 4096.f || mx > m + 12.f);
           if (kFp8 || look || !__any_sync(0xffffffffu, low)) break;
         }
         if (!ok) break;
