@@ -242,6 +242,18 @@ def test_rows_of_a_tile_without_a_sequence_change_nothing(H, HK, dtype, kv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("own", [(1,) * 40, (60, 300) * 20, (5, 900) * 60])
+def test_scales_that_change_right_before_the_call(own):
+    """v_scale comes from the launch just before: powers of two scale the result exactly."""
+    c = Case(own=own, prefix=4096, kv="fp8")
+    want = c.call().float()
+    for i in range(100):
+        f = 2.0 ** (i % 5 - 2)
+        c.vs.fill_(0.21 * f)
+        assert torch.equal(c.call().float(), want * f)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("kw", [dict(dtype="fp32"), dict(B=8), dict(own=(40,))])
 def test_shapes_without_a_kernel_run_as_ordinary_decodes(kw):
     c = Case(prefix=64, **kw)

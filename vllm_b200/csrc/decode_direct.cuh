@@ -434,7 +434,7 @@ __device__ __forceinline__ void decode_direct(const DecodeParams& p, const int c
 
   // ---- merges.  A unit is four head dimensions of one head.
   constexpr int UPH = D / 4;
-  const float kv_o = kFp8 ? *p.v_scale : 1.f;
+  const float kv_o = kFp8 ? (kBehind ? __ldcg(p.v_scale) : *p.v_scale) : 1.f;
   // (kBehind: a sum that is NaN is not left out)
   auto counts = [](float l) { return kBehind ? l != 0.f : l > 0.f; };
   if constexpr (kBehind) grid_dependency();  // (from here on the prefix's parts)

@@ -915,7 +915,7 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
 
   // fold the per-tensor scales of an fp8 cache into the logit scale and the output scale
   const float kv_qk = kFp8 ? (kBehind ? __ldcg(p.k_scale) : *p.k_scale) : 1.f;
-  const float kv_o = kFp8 ? *p.v_scale : 1.f;
+  const float kv_o = kFp8 && !kBehind ? *p.v_scale : 1.f;  // (kBehind: where the parts are added up)
   const float qk_scale = p.scale * kLog2e * kv_qk;
   bool failed = false;
   const bool has_alibi = p.alibi != nullptr;
