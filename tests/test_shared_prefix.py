@@ -225,6 +225,26 @@ def test_infinite_and_nan_keys_stay_with_their_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["auto", "fp8_e5m2"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("blocks", [range(256, 257), range(256, 258), range(257, 258), range(256, 264), range(0, 8),
+                                    range(8, 16), range(0, 256)], ids=lambda r: f"{r.start}-{r.stop}")
+def test_logits_of_minus_infinity(blocks, D, kv):
+    """Whole tiles, the whole prefix, and all own tokens (blocks from 256 on) with logits of -inf: weights of 0."""
+    c = Case(own=(20, 50, 100, 128, 7) * 12, prefix=4096, D=D, kv=kv)
+    if "B200PA_TUNE_BEHIND" not in os.environ:
+        assert _route(prefix=c.prefix, num_seqs=60, head_size=D, q_stride=8 * D, kv_block_stride=32 * D, kv_head_stride=16 * D,
+                      max_seq_len=c.max_len) != 0
+    c.q[:, :, 0] = c.q[:, :, 0].abs() + 0.25
+    for b in blocks:
+        for i in range(c.N):
+            if b * c.B < int(c.lens[i]):
+                c.kc[c.bt[i, b], :, 0, :, 0] = 0xFC if kv != "auto" else -float("inf")
+    lse = torch.full((c.H, c.N), 5.0, device=DEV)
+    c.check(c.call(lse=lse), lse)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("H,HK", [(28, 4), (12, 4), (40, 8)])
 @pytest.mark.parametrize("dtype,kv", [("bf16", "auto"), ("fp16", "fp8"), ("bf16", "fp8_e5m2")])
 def test_rows_of_a_tile_without_a_sequence_change_nothing(H, HK, dtype, kv):
