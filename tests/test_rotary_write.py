@@ -299,6 +299,35 @@ def test_refusals(what, kw, msg):
     assert (c.out == 3.0).all() and (c.kc == 7).all() and (c.vc == 7).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout,spoil", [
+    ("x", lambda v: v.view(-1, 2, 64, 32)), ("x", lambda v: v.view(-1, 2, 256, 8)), ("x", lambda v: v.view(-1, 1, 128, 32)),
+    ("x", lambda v: v[:-1]),
+    ("NHD", lambda v: v.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)),  # as HND in memory
+    ("HND", lambda v: v.contiguous()), ("NHD", lambda v: v.view(-1, 32, 1, 128)), ("NHD", lambda v: v.view(-1, 8, 4, 128)),
+    ("NHD", lambda v: v[:-1]),
+])
+def test_caches_of_two_layouts_are_refused(layout, spoil):
+    """As many elements, and blocks as far apart, but V's in other places than K's."""
+    c = Case(layout, ((0, 20),))
+    vc = spoil(c.vc)
+    with pytest.raises(RuntimeError, match="same|stride"):
+        c.call(value_cache=vc)
+    torch.cuda.synchronize()
+    assert (c.out == 3.0).all() and (c.kc == 7).all() and (vc == 7).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("layout", ["NHD", "HND"])
+def test_strides_of_dimensions_of_size_one_mean_nothing(layout):
+    """One kv head: NHD and HND caches are the same bytes, whatever strides they name."""
+    c = Case(layout, ((0, 20),), HK=1)
+    other = torch.full((c.nb, 1, c.B, c.D), 7, dtype=c.vc.dtype, device=DEV).transpose(1, 2)
+    c.vc = other if layout == "NHD" else other.contiguous().view(c.nb, c.B, 1, c.D)
+    c.call()
+    c.check()
+
+
 def _c_args(**kw):
     buf = C.create_string_buffer(1024)
     mem = C.addressof(buf) + 255 & ~255  # (any aligned address: nothing is launched)

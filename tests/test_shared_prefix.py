@@ -389,6 +389,30 @@ def test_refusals(what, kw, msg):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("which", ["V's blocks elsewhere", "fewer V blocks", "K in pieces", "V in pieces", "slopes"])
+def test_layouts_that_are_refused(which):
+    """V is read by K's strides."""
+    c = Case(own=(5, 9, 30, 1), prefix=144, alibi=True)
+    kw = {}
+    if which == "V's blocks elsewhere":
+        kw["value_cache"] = torch.stack([c.vc, c.vc], 1)[:, 0]
+    elif which == "fewer V blocks":
+        kw["value_cache"] = c.vc[:-1]
+    elif which == "K in pieces":
+        kw["key_cache"] = torch.stack([c.kc, c.kc], 4)[:, :, :, :, 0]
+        kw["value_cache"] = torch.stack([c.vc, c.vc], 1)[:, 0].as_strided(c.vc.shape, (*kw["key_cache"].stride()[:2], 16, 1))
+    elif which == "V in pieces":
+        kw["value_cache"] = c.vc.transpose(2, 3).contiguous().transpose(2, 3)
+    else:
+        kw["alibi_slopes"] = torch.stack([c.alibi, c.alibi], 1)[:, 0]
+    out = torch.full((c.N, c.H, c.D), 9.0, dtype=c.dtype, device=DEV)
+    with pytest.raises(RuntimeError, match="strides|alibi_slopes"):
+        c.call(out=out, **kw)
+    torch.cuda.synchronize()
+    assert (out == 9.0).all()
+
+
+@pytest.mark.gpu
 def test_the_c_interface_asks_for_scratch():
     c = Case(own=(5, 9, 30) * 20, prefix=4096)
     out = torch.full((c.N, c.H, c.D), 9.0, dtype=c.dtype, device=DEV)

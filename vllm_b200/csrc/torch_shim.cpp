@@ -226,6 +226,14 @@ bool paged_attention_varlen(torch::Tensor& out, torch::Tensor& query, torch::Ten
   return true;
 }
 
+// Whether the first `dims` dimensions of K's cache and V's have the same sizes and strides (the stride of a dimension
+// of size 1 means nothing).
+bool same_layout(const torch::Tensor& k, const torch::Tensor& v, int dims) {
+  for (int i = 0; i < dims; ++i)
+    if (k.size(i) != v.size(i) || (k.size(i) > 1 && k.stride(i) != v.stride(i))) return false;
+  return true;
+}
+
 // Decode attention over a prefix that the sequences share (not an op of the reference).
 void paged_attention_shared_prefix(torch::Tensor& out, torch::Tensor& query, torch::Tensor& key_cache,
                                    torch::Tensor& value_cache, int64_t num_kv_heads, double scale,
@@ -245,8 +253,19 @@ void paged_attention_shared_prefix(torch::Tensor& out, torch::Tensor& query, tor
                   key_cache.size(3) == block_size && value_cache.size(1) == num_kv_heads && value_cache.size(2) == D &&
                   value_cache.size(3) == block_size,
               "the caches do not have these heads, head size and block size");
+  // (V is read by K's strides, and a block of a head is one piece)
+  auto one_piece = [](const torch::Tensor& t) {
+    int64_t n = 1;
+    for (int64_t i = t.dim() - 1; i >= 2; n *= t.size(i--))
+      if (t.size(i) > 1 && t.stride(i) != n) return false;
+    return true;
+  };
+  TORCH_CHECK(same_layout(key_cache, value_cache, 2) && one_piece(key_cache) && one_piece(value_cache),
+              "key_cache and value_cache must have the same strides between blocks and heads, and nothing in between "
+              "inside a block of a head");
   TORCH_CHECK(prefix_len >= 0 && prefix_len <= INT32_MAX, "prefix_len ", prefix_len, " is out of range");
-  TORCH_CHECK(!alibi_slopes.has_value() || alibi_slopes->numel() == query.size(1), "alibi_slopes must be [num_heads]");
+  TORCH_CHECK(!alibi_slopes.has_value() || (alibi_slopes->numel() == query.size(1) && alibi_slopes->is_contiguous()),
+              "alibi_slopes must be [num_heads], contiguous");
   const auto dev = query.device();
   for (const torch::Tensor* t : {&out, &key_cache, &value_cache, &block_tables, &seq_lens})
     TORCH_CHECK(t->device() == dev, "all tensors must be on one device");
@@ -393,8 +412,12 @@ void rotary_write(torch::Tensor& query_out, torch::Tensor& positions, torch::Ten
               cos_sin_cache.size(1), " has to be even and at most the head size ", D);
   const int64_t cache_heads = flash ? key_cache.size(2) : key_cache.size(1);
   const int64_t cache_dim = flash ? key_cache.size(3) : key_cache.size(2) * key_cache.size(4);
-  TORCH_CHECK(cache_heads == key.size(1) && cache_dim == D && value_cache.numel() == key_cache.numel(),
-              "the caches do not have the key's heads and head size");
+  TORCH_CHECK(cache_heads == key.size(1) && cache_dim == D, "the caches do not have the key's heads and head size");
+  // (V goes to the places that K's strides give)
+  TORCH_CHECK(flash ? same_layout(key_cache, value_cache, 4)
+                    : value_cache.size(0) == key_cache.size(0) && value_cache.size(1) == cache_heads &&
+                          value_cache.size(2) == D && value_cache.size(3) == key_cache.size(3),
+              "key_cache and value_cache must have the same blocks, heads, head size, block size and strides");
   for (const torch::Tensor* t : {&query_out, &positions, &query, &value, &cos_sin_cache, &key_cache, &value_cache, &slot_mapping})
     TORCH_CHECK(t->device() == key.device(), "all tensors must be on one device");
   TORCH_CHECK(a.kv_dtype == B200PA_KV_AUTO || (k_scale.device() == key.device() && v_scale.device() == key.device()),
