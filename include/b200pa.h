@@ -301,7 +301,8 @@ int b200pa_reshape_and_cache_flash(const b200pa_cache_args* args, void* stream);
  * in the reference's paged-attention ops).  The arithmetic is fp32, rounded once: to the query's type for
  * query_out and 16/32-bit caches, to the code of k / k_scale for fp8 caches.
  *   query_out, query  [num_tokens, num_heads, head_size], row strides query_out_stride / query_stride; the
- *                     same tensor (pointer and stride) for a rotation in place, else without overlap
+ *                     same tensor (pointer and stride) for a rotation in place, else without overlap (refused;
+ *                     key and value must not lie in query_out either)
  *   positions         [num_tokens] int64
  *   cos_sin           [max_position, rot_dim] contiguous: cosines of rot_dim / 2 pairs, then their sines;
  *                     float32 or of the query's type (table_dtype)

@@ -356,6 +356,40 @@ def test_the_c_interface_refuses(kw, msg):
     assert capi.launch_count() == 0
 
 
+@pytest.mark.parametrize("out,stride", [(8, 512), (-8, 512), (512, 512), (-512, 512), (0, 520), (511, 2048),
+                                        (4096, 512), (4097 - 512, 512), (4096 + 255, 512), (8192, 512), (8192 - 1024, 1024)])
+def test_the_c_interface_refuses_a_query_out_over_its_inputs(out, stride):
+    """Element offsets of query_out: over query (rows of 512 from 0 on, 2048 apart), key (256 from 4096) and value (from
+    8192), 3 rows each.  (Nothing runs: the addresses are the test's own.)"""
+    r, a, buf = _c_args()
+    base = r.query
+    a.key, a.value = base + 2 * 4096 * 2, base + 2 * 8192 * 2
+    r.query_stride = 2048 if stride == 2048 else 512
+    r.query_out, r.query_out_stride = base + 2 * out, stride
+    if out >= 4096 - 512:
+        a.key, a.value = base + 2 * 4096, base + 2 * 8192
+    capi.launch_count(reset=True)
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        capi.rotary_reshape_and_cache(r, a)
+    assert capi.launch_count() == 0
+
+
+@pytest.mark.gpu
+def test_outputs_beside_the_inputs():
+    """query_out in the same buffer as the projection's output, in columns of its own: no overlap."""
+    for H, HK in ((4, 2), (8, 1)):
+        c = Case("x", ((0, 70), (5, 1)), H=H, HK=HK)
+        n, w = c.slots.numel(), (H + 2 * HK) * c.D
+        buf = torch.randn(n, w + H * c.D, device=DEV).to(c.dtype)
+        buf[:, :w] = torch.cat([c.q, c.k, c.v], 1).view(n, w)
+        parts = buf.split([H * c.D, HK * c.D, HK * c.D, H * c.D], 1)
+        c.q, c.k, c.v, out = (t.view(n, -1, c.D) for t in parts)
+        c.call(out=out)
+        c.check(out=out)
+        with pytest.raises(RuntimeError, match="must not overlap"):
+            c.call(out=buf[:, c.D:].split(H * c.D, 1)[0].view(n, H, c.D))
+
+
 def test_the_c_interface_takes_nothing_to_do():
     r, a, _ = _c_args(num_tokens=0, query=None, key=None)
     capi.rotary_reshape_and_cache(r, a)

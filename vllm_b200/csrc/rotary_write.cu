@@ -475,6 +475,21 @@ static int dispatch_rotary(const RotaryParams& p, int kv_dtype, cudaStream_t s) 
   return B200PA_EUNSUPPORTED;
 }
 
+// Whether two tensors of `rows` rows share bytes (rows of `bytes`, `stride` apart).  Of different strides only their
+// extents are compared.
+struct RowSpan {
+  const void* ptr;
+  int64_t stride, bytes;
+};
+static bool rows_meet(const RowSpan& a, const RowSpan& b, int64_t rows) {
+  const uintptr_t pa = reinterpret_cast<uintptr_t>(a.ptr), pb = reinterpret_cast<uintptr_t>(b.ptr);
+  if (pa + (rows - 1) * a.stride + a.bytes <= pb || pb + (rows - 1) * b.stride + b.bytes <= pa) return false;
+  if (rows == 1 || a.stride != b.stride || a.stride < a.bytes || b.stride < b.bytes) return true;
+  int64_t d = int64_t(pb - pa) % a.stride;  // of b's rows inside a's
+  if (d < 0) d += a.stride;
+  return d < a.bytes || d + b.bytes > a.stride;
+}
+
 static int rotary_entry(const b200pa_rotary_args* r, const b200pa_cache_args* a, void* stream, bool flash) {
   B200PA_CHECK_ARG(r != nullptr && a != nullptr, "args is NULL");
   B200PA_CHECK_ARG(a->num_tokens >= 0 && a->num_heads > 0 && a->head_size > 0 && a->block_size > 0 && r->num_heads > 0,
@@ -503,6 +518,14 @@ static int rotary_entry(const b200pa_rotary_args* r, const b200pa_cache_args* a,
                        a->value_cache && a->slot_mapping,
                    "null tensor pointer");
   B200PA_CHECK_ARG(a->kv_dtype == B200PA_KV_AUTO || (a->k_scale && a->v_scale), "fp8 kv cache needs k_scale and v_scale");
+  const int64_t es = a->in_dtype == B200PA_F32 ? 4 : 2, n = a->num_tokens, q_row = int64_t(r->num_heads) * a->head_size * es,
+                kv_row = int64_t(a->num_heads) * a->head_size * es;
+  const RowSpan out{r->query_out, r->query_out_stride * es, q_row};
+  const bool in_place = r->query_out == r->query && (n == 1 || r->query_out_stride == r->query_stride);
+  B200PA_CHECK_ARG((in_place || !rows_meet(out, {r->query, r->query_stride * es, q_row}, n)) &&
+                       !rows_meet(out, {a->key, a->key_stride * es, kv_row}, n) &&
+                       !rows_meet(out, {a->value, a->value_stride * es, kv_row}, n),
+                   "query_out must not overlap key, value, or query (but for a rotation in place)");
   RotaryParams p{};
   p.query_out = r->query_out;
   p.query = r->query;
