@@ -157,3 +157,44 @@ def test_key_and_value_go_together():
     q = torch.zeros(1, 8, 128)
     with pytest.raises(AssertionError, match="go together"):
         impl.forward(None, q, q, None, None, md, output=torch.zeros(1, 1024))
+
+
+@pytest.mark.gpu
+def test_keys_behind_the_rotation_are_refused():
+    """forward would write the unrotated keys over the rotated ones; the step after it may bring its own again."""
+    s = Session(3, 64, [4, 9, 1])
+    s.step([1] * 3)
+    n = 3
+    q, k, v = (torch.randn(n, h, s.D, generator=s.g).to(s.dtype).to(DEV) for h in (s.H, s.HK, s.HK))
+    slots = (s.table[:, -1].long() * s.B).to(DEV)
+    md = s.builder.build(0, types.SimpleNamespace(
+        query_start_loc=torch.arange(4, dtype=torch.int32, device=DEV), seq_lens=s.lens.int().to(DEV), num_reqs=n,
+        num_actual_tokens=n, max_query_len=1, max_seq_len=int(s.lens.max()), block_table_tensor=s.table, slot_mapping=slots))
+    out = torch.full((n, s.H * s.D), 7.0, dtype=s.dtype, device=DEV)
+    s.impl.do_rope_and_kv_cache_update(s.layer, q, k, v, s.lens.to(DEV), s.rope, True, s.cache, slots)
+    cache = s.cache.clone()
+    with pytest.raises(ValueError, match="key and value None"):
+        s.impl.forward(s.layer, q, k, v, s.cache, md, output=out)
+    torch.cuda.synchronize()
+    assert torch.equal(s.cache, cache) and (out == 7.0).all()
+    s.impl.do_rope_and_kv_cache_update(s.layer, q, k, v, s.lens.to(DEV), s.rope, True, s.cache, slots)
+    s.impl.forward(s.layer, q, None, None, s.cache, md, output=out)
+    s.impl.forward(s.layer, q, k, v, s.cache, md, output=out)
+
+
+def test_keys_behind_the_rotation_are_refused_on_the_host(monkeypatch):
+    impl = B200PagedAttentionImpl(8, 128, 0.1, 2)
+    monkeypatch.setattr(PagedAttention, "rotate_and_write_to_paged_cache", lambda *a, **k: None)
+    monkeypatch.setattr(ops, "attention_step", lambda *a: True)
+    q, kv = torch.zeros(1, 8, 128), torch.zeros(1, 2, 128)
+    md = types.SimpleNamespace(num_actual_tokens=1, num_decodes=1, max_query_len=1, max_seq_len=4, use_cascade=False,
+                               block_table=None, seq_lens=None, slot_mapping=None, query_start_loc=None, common_prefix_len=0)
+    layer = types.SimpleNamespace(_k_scale=None, _v_scale=None)
+    cache, out = torch.zeros(2, 1, 16 * 2 * 128), torch.zeros(1, 1024)
+    rotate = lambda: impl.do_rope_and_kv_cache_update(layer, q, kv, kv, None, None, True, cache, torch.zeros(1))  # noqa: E731
+    rotate()
+    with pytest.raises(ValueError, match="key and value None"):
+        impl.forward(layer, q, kv, kv, cache, md, output=out)
+    rotate()
+    assert impl.forward(layer, q, None, None, cache, md, output=out) is out
+    assert impl.forward(layer, q, kv, kv, cache, md, output=out) is out  # the next step, without the rotation

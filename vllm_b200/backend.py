@@ -159,6 +159,7 @@ class B200PagedAttentionImpl:
         self.kv_cache_dtype = kv_cache_dtype
         self.kv_sharing_target_layer_name = kv_sharing_target_layer_name
         self.num_queries_per_kv = num_heads // num_kv_heads
+        self.cache_written = False  # by do_rope_and_kv_cache_update, for the next forward
 
     def fused_rope_kvcache_supported(self) -> bool:
         return self.kv_sharing_target_layer_name is None
@@ -167,12 +168,14 @@ class B200PagedAttentionImpl:
                                     positions: torch.Tensor, cos_sin_cache: torch.Tensor, is_neox: bool,
                                     kv_cache: torch.Tensor, slot_mapping: torch.Tensor) -> None:
         """Rotates `query` in place and writes the rotated `key` and `value` to the cache, in one launch
-        (``rotary_reshape_and_cache``); `key` stays as it is.  `forward` is called with ``key`` and
-        ``value`` None then."""
+        (``rotary_reshape_and_cache``); `key` stays as it is.  Who calls this calls `forward` with ``key``
+        and ``value`` None then; with them it would write the unrotated key over the rotated one, and
+        raises ValueError instead."""
         key_cache, value_cache = PagedAttention.split_kv_cache(kv_cache, self.num_kv_heads, self.head_size)
         PagedAttention.rotate_and_write_to_paged_cache(
             query, key, value, positions, cos_sin_cache, is_neox, key_cache, value_cache, slot_mapping,
             self.kv_cache_dtype, layer._k_scale, layer._v_scale, query_out=query)
+        self.cache_written = True
 
     def forward(self, layer, query: torch.Tensor, key: torch.Tensor | None, value: torch.Tensor | None,
                 kv_cache: torch.Tensor, attn_metadata: B200PagedAttentionMetadata | None,
@@ -189,6 +192,10 @@ class B200PagedAttentionImpl:
         md = attn_metadata
         n = md.num_actual_tokens
         assert (key is None) == (value is None), "key and value go together"
+        written, self.cache_written = self.cache_written, False
+        if written and key is not None:
+            raise ValueError("do_rope_and_kv_cache_update has written this step's keys and values: call forward with "
+                             "key and value None")
         write = key is not None and self.kv_sharing_target_layer_name is None
         alibi = self.alibi_slopes
         if alibi is not None and alibi.device != query.device:
