@@ -198,3 +198,71 @@ def test_keys_behind_the_rotation_are_refused_on_the_host(monkeypatch):
     rotate()
     assert impl.forward(layer, q, None, None, cache, md, output=out) is out
     assert impl.forward(layer, q, kv, kv, cache, md, output=out) is out  # the next step, without the rotation
+
+
+def _taken(monkeypatch):
+    """What ops.attention_step answers, and the launches of it."""
+    from vllm_b200 import capi
+    step, taken = ops.attention_step, []
+
+    def record(*args):
+        capi.launch_count(reset=True)
+        done = step(*args)
+        taken.append((done, capi.launch_count()))
+        return done
+    monkeypatch.setattr(ops, "attention_step", record)
+    return taken
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,prefix", [(2, 16), (2, 256), (64, 16), (256, 16), (12, 64)])
+@pytest.mark.parametrize("chunks", [0, 2])
+def test_too_little_to_share_is_an_ordinary_step(monkeypatch, N, prefix, chunks):
+    """A cascade step whose sizes leave nothing to share: the same native call, the same launches, the same bits."""
+    taken = _taken(monkeypatch)
+    s = Session(N + chunks, prefix, [1 + 3 * i % 50 for i in range(N + chunks)])
+    md = s.step([1] * N + [9] * chunks)
+    assert md.use_cascade
+    out = [torch.empty((md.num_actual_tokens, s.H * s.D), dtype=s.dtype, device=DEV) for _ in range(2)]
+    q = torch.randn((md.num_actual_tokens, s.H, s.D), generator=s.g).to(s.dtype).to(DEV)
+    for o, shares in zip(out, (True, False)):
+        md.use_cascade = shares
+        s.impl.forward(s.layer, q, None, None, s.cache, md, output=o)
+    assert taken[0] == taken[1] == taken[2] and taken[0][0]
+    assert torch.equal(*out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[1] * 40, [1] * 40 + [30, 200]], ids=["decodes", "chunks"])
+@pytest.mark.parametrize("write", [True, False])
+def test_a_cascade_is_one_native_call(monkeypatch, new, write):
+    """The write, the shared prefix and the chunks go with the step's call: as the operators one by one, to the last bit."""
+    s = Session(len(new), 2048, [5 + 3 * i for i in range(len(new))])
+    md = s.step(new)
+    n = md.num_actual_tokens
+    q, k, v = (torch.randn((n, h, s.D), generator=s.g).to(s.dtype).to(DEV) for h in (s.H, s.HK, s.HK))
+    cache, taken = s.cache.clone(), _taken(monkeypatch)
+    out = [torch.full((n + 3, s.H * s.D), 7.0, dtype=s.dtype, device=DEV) for _ in range(2)]
+    kv = (k, v) if write else (None, None)
+    s.impl.forward(s.layer, q, *kv, s.cache, md, output=out[0])
+    done, launches = taken[0]
+    assert done and launches > 1 + write + (len(new) > 40)
+    monkeypatch.setattr(ops, "attention_step", lambda *args: False)
+    s.impl.forward(s.layer, q, *kv, cache, md, output=out[1])
+    assert torch.equal(*out) and torch.equal(s.cache, cache)
+    assert (out[0][n:] == 7.0).all()
+
+
+def test_the_step_is_told_the_prefix(monkeypatch):
+    seen = []
+    monkeypatch.setattr(ops, "attention_step", lambda *a: seen.append(a[-1]) or True)
+    impl = B200PagedAttentionImpl(8, 128, 0.1, 2)
+    q, out = torch.zeros(3, 8, 128), torch.zeros(3, 1024)
+    layer = types.SimpleNamespace(_k_scale=None, _v_scale=None)
+    b = B200PagedAttentionMetadataBuilder(16)
+    common = types.SimpleNamespace(
+        query_start_loc=torch.arange(4), seq_lens=torch.tensor([70, 90, 80]), num_reqs=3, num_actual_tokens=3,
+        max_query_len=1, max_seq_len=90, block_table_tensor=torch.zeros(3, 6), slot_mapping=torch.zeros(3))
+    for prefix in (64, 0):
+        impl.forward(layer, q, None, None, torch.zeros(2, 6, 4096), b.build(prefix, common), output=out)
+    assert seen == [64, 0]

@@ -207,14 +207,15 @@ class B200PagedAttentionImpl:
         if md.max_query_len > 1 and torch.cuda.is_current_stream_capturing():
             num_decodes = 0
         cascade = md.use_cascade and num_decodes > 1
-        if not cascade and ops.attention_step(
+        # (whether the decodes share the prefix in fact is decided there, by the sizes of the batch)
+        if ops.attention_step(
                 output, query, key, value, kv_cache, md.block_table, md.seq_lens, md.slot_mapping,
                 md.query_start_loc, layer._k_scale, layer._v_scale, alibi, n, num_decodes,
                 md.max_query_len, md.max_seq_len, self.num_heads, self.num_kv_heads, self.head_size,
                 self.scale, self.kv_cache_dtype, write,
-                PagedAttention.use_v1(md.max_seq_len, n, self.num_heads)):
+                PagedAttention.use_v1(md.max_seq_len, n, self.num_heads), md.common_prefix_len if cascade else 0):
             return output
-        # a cascade step, or not a plain call (fp32, odd strides, tracing, ...): operator by operator
+        # not a plain call (fp32, odd strides, tracing, ...): operator by operator
         key_cache, value_cache = PagedAttention.split_kv_cache(kv_cache, self.num_kv_heads,
                                                                self.head_size)
         if write:
@@ -293,8 +294,9 @@ class B200PagedAttentionBackend:
                               use_local_attention: bool = False, num_sms: int = 0, dcp_world_size: int = 1,
                               **kwargs) -> bool:
         """Whether a step with this common prefix is built as a cascade: there are decodes to share it
-        (``query_lens``: new tokens of the requests, the single ones in front).  Which kernels it runs on -
-        the ordinary ones where there is too little to share - is decided from the sizes of the batch."""
+        (``query_lens``: new tokens of the requests, the single ones in front).  Which kernels it runs on is
+        decided by `forward`, which knows all sizes: where there is too little to share it is an ordinary
+        step in every respect."""
         if common_prefix_len <= 0 or query_lens is None or use_sliding_window or use_local_attention:
             return False
         return dcp_world_size == 1 and len(query_lens) > 1 and int(query_lens[0]) == int(query_lens[1]) == 1

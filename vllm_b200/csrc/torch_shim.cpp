@@ -927,6 +927,7 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const double scale = in.real();
   const std::string kv = in.text();
   const int64_t write = in.integer(), prefer_v1 = in.integer();
+  const int64_t prefix = in.integer();  // tokens that all requests begin with, in the same blocks; 0: none
   return direct(in, [&]() -> bool {
     using at::ScalarType;
     const auto type = q.scalar_type();
@@ -1016,6 +1017,27 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       c.head_size = static_cast<int32_t>(D);
       c.block_size = static_cast<int32_t>(B);
       c.x = static_cast<int32_t>(x);
+    }
+    // a cascade, where the sizes of the leading decodes leave something to share; else an ordinary step
+    const int64_t sharing = max_q == 1 ? tokens : std::min(decodes, tokens);
+    if (prefix > 0 && sharing > 1) {
+      b200pa_attn_args d = p;
+      d.num_seqs = static_cast<int32_t>(sharing);
+      const int32_t length = static_cast<int32_t>(std::min<int64_t>(prefix, INT32_MAX));
+      int32_t way = 0;
+      if (b200pa_shared_prefix_route(&d, length, &way) != B200PA_OK) return false;
+      if (way != 0) {
+        const int64_t bytes = b200pa_shared_prefix_scratch_bytes(&d, length);
+        const at::Tensor scratch = at::empty({bytes}, q.options().dtype(ScalarType::Byte));
+        if (write) check_rc(b200pa_reshape_and_cache(&c, stream));
+        check_rc(b200pa_paged_attention_shared_prefix(&d, length, scratch.data_ptr(), bytes, stream));
+        if (max_q == 1 || decodes >= reqs) return true;
+        p.num_seqs = static_cast<int32_t>(reqs - decodes);
+        p.block_tables += decodes * p.max_num_blocks_per_seq;
+        p.seq_lens += decodes;
+        check_rc(b200pa_paged_attention_varlen(&p, qsl.data_ptr<int>() + decodes, static_cast<int32_t>(tokens), 0, stream));
+        return true;
+      }
     }
     auto run = [&](const int* starts, bool caller_scratch) {
       check_rc(b200pa_attention_step(write ? &c : nullptr, &p, starts, static_cast<int32_t>(tokens),
