@@ -92,6 +92,11 @@ static int64_t unit_ns(int head_size, int row_tiles, int turns, bool biased, boo
   return std::max(work, tile_bytes * 1000 / 60000);
 }
 
+// ... and for a piece of an item beside its key tiles: a pipeline that fills and drains, queries in, a part out.  (A prefix
+// of 96 tokens is one key tile: without this its CTAs were last.  1029 sequences behind 96, 8 / 2 heads of 128, 115 -> 95
+// us; 430 behind 96, 28 / 4 heads of 256, 246 -> 162; 256 behind 256, 32 / 8 heads of 128, 131 -> 97.)
+static int64_t piece_ns(int head_size, int turns) { return (2500 + 14 * head_size) / (turns ? 2 : 1); }
+
 // Which way a call goes: 0 the ordinary kernels on whole sequences; behind the prefix the direct kernel (1), the same
 // with a warp to an item (2), or the persistent one beside the prefix and a third launch (3).  What each takes, us:
 // fitted to 410 random batches (2 to 2000 sequences, prefixes of 64 to 65000 tokens, up to 3000 own ones, all head sizes,
@@ -172,7 +177,7 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
     r.grid = sms;
     const int64_t page = int64_t(a.head_size) * a.block_size * es * 2;  // bytes of a block and kv head
     r.balance.sms = sms;
-    r.balance.prefix = units * unit;
+    r.balance.prefix = units * unit + items * piece_ns(a.head_size, r.turns);
     r.balance.items = tail_items * 500;
     if (tune.prefix) r.balance.prefix = r.balance.prefix * tune.prefix / 100;
     r.balance.block = page * 1000 / 65000;
