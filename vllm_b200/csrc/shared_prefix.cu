@@ -100,8 +100,9 @@ static int64_t piece_ns(int head_size, int turns) { return (2500 + 14 * head_siz
 // Which way a call goes: 0 the ordinary kernels on whole sequences; behind the prefix the direct kernel (1), the same
 // with a warp to an item (2), or the persistent one beside the prefix and a third launch (3).  What each takes, us:
 // fitted to 410 random batches (2 to 2000 sequences, prefixes of 64 to 65000 tokens, up to 3000 own ones, all head sizes,
-// cache types and ten head counts; own lengths are taken as half the bound).  The choice is 2.3 % from the best of the
-// four on average, more than 25 % in 7 cases (on 150 others 3.6 %, in 6); each of them alone 81, 23, 87 and 52 %.
+// cache types and ten head counts; own lengths are taken as half the bound).  Over these and 500 others the choice is
+// 3.3 % from the best of the four on average, more than 25 % in 35 of the 910.  The ordinary kernels are given 5 %: that
+// costs nothing on average, and 32 of the 910 are over 10 % slower than them, not 48.
 //   prefix_all: the prefix's work over all SMs; prefix_cut: of its longest CTA
 static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const SharedPrefixPlan& r, double prefix_all,
                              double prefix_cut, bool tails) {
@@ -126,6 +127,7 @@ static int shared_prefix_way(const b200pa_attn_args& a, int prefix_len, const Sh
   const double tail_items = N * a.num_kv_heads * ((group + (group <= 8 ? 7 : 15)) / (group <= 8 ? 8 : 16));
   const double beside = (N * own / 2 * row / 65e3 + tail_items * 0.5) / sms;
   t[3] = tails ? 25 + std::max(prefix_all + beside, hbm) + 0.6e-6 * N * a.num_heads * D * 4 : 1e30;
+  t[0] *= 0.95;
   return int(std::min_element(t, t + 4) - t);
 }
 
