@@ -151,6 +151,14 @@ def test_long_and_uneven_own_parts(kv):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kv", ["auto", "fp8"])
+def test_one_long_sequence_among_short_ones(kv):
+    """Its own part is cut over nearly all warps, into as many pieces as there may be."""
+    _run(prefix=1024, own=(30000,) + tuple(1 + 7 * i % 100 for i in range(60)), kv=kv, H=8, HK=1)
+    _run(prefix=2048, own=(3, 9000, 12, 9000) + (20,) * 60, kv=kv, H=16, HK=2, D=64)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype,kv", [("bf16", "auto"), ("fp16", "fp8")])
 @pytest.mark.parametrize("N", [4, 40])
 def test_alibi(dtype, kv, N):

@@ -626,14 +626,14 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
       // Range length: an equal share for every warp of the grid, at least the smallest range
       // worth a work item, and large enough that the longest sequence is cut into no more
       // pieces than the scratch has slots per sequence (a sequence of n units meets at most
-      // (n - 1) / C + 2 ranges).  Even, see above.
+      // (n - 1) / C + 2 ranges; kBehind: than the third launch should add up).  Even, see above.
       const long long U = (long long)hsubs * total;
       const int ctas = kBehind ? pre.balance.sms - pre.balance.prefix_ctas(U) : int(gridDim.x);
       if (kBehind) s_plan[3] = ctas;
       const long long W = (long long)ctas * nwarps;
       long long C = (U + W - 1) / W;
       C = max(C, (long long)p.min_chunk);
-      if (!kBehind) C = max(C, (long long)((n_max - 1) / max(1, p.max_partitions - 1) + 1));
+      C = max(C, (long long)((n_max - 1) / max(1, p.max_partitions - 1) + 1));
       C = (C + 1) & ~1ll;
       s_plan[0] = int(min(C, (long long)INT32_MAX - 1));
       s_plan[1] = total;

@@ -65,6 +65,12 @@ static bool plan_tails(const b200pa_attn_args& a, int gp, SharedPrefixPlan& r) {
   return true;
 }
 
+// Pieces that the persistent kernel cuts a sequence into, at most: the third launch adds them up four at a time, a trip to
+// memory each.  One sequence of 30000 own tokens among 256 behind 1024 tokens, 8 / 1 heads of 128: without a bound (469
+// pieces of 64 tokens) 74 us, 256 pieces 55, 128 58, 64 81 (the warps with them are last then); 32 / 8 heads 81 with 96
+// and more.
+constexpr int kMostPieces = 256;
+
 static SharedPrefixKernels find_shared_prefix(const b200pa_attn_args& a) {
   const int es = a.kv_dtype == B200PA_KV_AUTO ? 2 : 1;
   auto al = [](const void* ptr) { return reinterpret_cast<uintptr_t>(ptr) % 16 == 0; };
@@ -315,6 +321,7 @@ extern "C" int b200pa_paged_attention_shared_prefix(const b200pa_attn_args* args
     d.nstages = plan.slots;
     d.use_table = 1;
     d.min_chunk = plan.min_chunk;
+    d.max_partitions = tuning().max_parts ? tuning().max_parts : kMostPieces;  // (bounds the cuts)
     pre.own = p.parts + plan.own_at;
     pre.found = reinterpret_cast<int2*>(p.parts + plan.found_at);
     pre.balance = plan.balance;
