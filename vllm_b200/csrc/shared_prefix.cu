@@ -101,7 +101,7 @@ static int64_t unit_ns(int head_size, int row_tiles, int turns, bool biased, boo
 // ... and for a piece of an item beside its key tiles: a pipeline that fills and drains, queries in, a part out.  (A prefix
 // of 96 tokens is one key tile: without this its CTAs were last.  1029 sequences behind 96, 8 / 2 heads of 128, 115 -> 95
 // us; 430 behind 96, 28 / 4 heads of 256, 246 -> 162; 256 behind 256, 32 / 8 heads of 128, 131 -> 97.)
-static int64_t piece_ns(int head_size, int turns) { return (2500 + 14 * head_size) / (turns ? 2 : 1); }
+static int64_t piece_ns(int head_size, int turns) { return turns ? 0 : 2500 + 14 * head_size; }
 
 // Which way a call goes: 0 the ordinary kernels on whole sequences; behind the prefix the direct kernel (1), the same
 // with a warp to an item (2), or the persistent one beside the prefix and a third launch (3).  What each takes, us:
