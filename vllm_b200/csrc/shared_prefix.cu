@@ -94,7 +94,7 @@ static SharedPrefixKernels find_shared_prefix(const b200pa_attn_args& a) {
 static int64_t unit_ns(int head_size, int row_tiles, int turns, bool biased, bool fp8, int64_t tile_bytes) {
   int64_t work = row_tiles == 1 ? 1800 : turns ? 1000 + 4 * head_size : 1500 + 8 * std::min(head_size, 128);
   if (biased) work = work * 3 / 2;
-  else if (fp8 && !turns) work = work * 17 / 20;
+  else if (fp8 && !turns) work = work * 41 / 50;
   return std::max(work, tile_bytes * 1000 / 60000);
 }
 
