@@ -511,3 +511,22 @@ def test_what_needs_scratch():
     assert need(**many, kv_head_stride=0) == 0 and need(**many, num_kv_heads=1, kv_head_stride=0) > 0
     part = 128 * (128 * 4 + 8)
     assert need(num_seqs=64, prefix=4096, max_num_blocks_per_seq=300) >= 2 * part
+
+
+@pytest.mark.skipif("B200PA_TUNE_BEHIND" in os.environ, reason="forced")
+@pytest.mark.parametrize("H,HK", [(40, 40), (16, 8), (24, 8), (40, 8), (32, 4), (64, 4)])
+def test_partials_have_room_for_the_heads_that_there_are(H, HK):
+    """Where the persistent kernel is behind the prefix: a partial of an item's heads to every item, and one more to every
+    range (12 to 16 warps of 148 SMs at most), beside the prefix's parts."""
+    N, D, prefix = 300, 128, 4096
+    kw = dict(num_seqs=N, num_heads=H, num_kv_heads=HK, q_stride=H * D, kv_block_stride=HK * D * 16, kv_head_stride=D * 16,
+              max_num_blocks_per_seq=400, max_seq_len=prefix + 1000)
+    assert _route(prefix=prefix, **(kw)) == 3
+    a, _ = _c_args(**kw)
+    group = H // HK
+    heads = min(group, 8 if group <= 8 else 16)
+    items = N * HK * -(-group // heads)
+    tiles = 2 * HK * -(--(-N // (128 // group)) // 2)
+    prefix_parts = (tiles + 2 * 148) * 128 * (D * 4 + 8)
+    own = (items + 16 * 148) * (heads * D * 4 + -(-heads * 8 // 16) * 16)
+    assert capi.shared_prefix_scratch_bytes(a, prefix) <= prefix_parts + own + items * 8 + 4096

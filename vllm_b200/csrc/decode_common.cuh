@@ -93,6 +93,12 @@ __device__ __forceinline__ int behind_prefix(int len, int prefix_len) {
   return len >= prefix_len ? len - prefix_len : max(len, 0);
 }
 
+// Bytes of a partial that the persistent kernel leaves behind a shared prefix: O of `heads` heads as [4 dimensions][heads]
+// in fp32, then (m, l) of the heads, up to a 16-byte boundary.
+__host__ __device__ constexpr int64_t own_part_bytes(int heads, int D) {
+  return int64_t(heads) * D * 4 + ((heads * 8 + 15) & ~15);
+}
+
 // What the launch in front has of a prefix that all sequences share (shared_prefix_kernel.cuh): which part of
 // it covers what, for the kernels that have the sequences' own tokens and add the prefix to them.
 struct SharedPrefixParts {

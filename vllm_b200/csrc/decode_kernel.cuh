@@ -1244,11 +1244,11 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
     // ---- finalise the item: l over the 8 row groups, normalise, write
     const bool direct = cur.nparts == 1;
     if constexpr (kBehind) {
-      // the piece's part, as the prefix's: O as [4 dimensions][heads] in fp32, then (m, l) of the heads
-      constexpr int HPI = TR::kHeadsPerItem;
+      // the piece's part (see own_part_bytes), with room for the heads that an item can have
+      const int room = min(TR::kHeadsPerItem, p.group);
       const int64_t item = int64_t(cur.kvh * p.head_groups + cur.hg) * p.num_seqs + cur.seq;
       if (cur.part == 0 && lane == 0) pre.found[item] = make_int2(int(my_number), cur.nparts);
-      float* own = reinterpret_cast<float*>(pre.own + (item + my_number) * (HPI * (D * 4 + 8)));
+      float* own = reinterpret_cast<float*>(pre.own + (item + my_number) * own_part_bytes(room, D));
 #pragma unroll
       for (int nt = 0; nt < GP; ++nt)
 #pragma unroll
@@ -1259,12 +1259,12 @@ __device__ __forceinline__ void decode_persistent(const DecodeParams& p, const S
           l += __shfl_xor_sync(0xffffffffu, l, 16);
           const int hl = nt * 8 + 2 * c + j;
           if (hl >= nheads) continue;
-          if (g == 0) reinterpret_cast<float2*>(own + HPI * D)[hl] = make_float2(m_run[nt][j], l);
+          if (g == 0) reinterpret_cast<float2*>(own + room * D)[hl] = make_float2(m_run[nt][j], l);
 #pragma unroll
           for (int mt = 0; mt < KS; ++mt) {
-            float* at = own + ((4 * mt + (g >> 2)) * HPI + hl) * 4 + (g & 3);
+            float* at = own + ((4 * mt + (g >> 2)) * room + hl) * 4 + (g & 3);
             at[0] = o[mt][nt][j];
-            at[2 * HPI * 4] = o[mt][nt][2 + j];
+            at[2 * room * 4] = o[mt][nt][2 + j];
           }
         }
     } else {

@@ -178,7 +178,7 @@ static SharedPrefixPlan shared_prefix_plan(const b200pa_attn_args& a, int prefix
   if (r.tails.fn != nullptr) {
     r.items = tail_items;
     r.heads = heads;
-    const int64_t slot = heads * (a.head_size * 4 + 8), ranges = int64_t(sms) * r.warps;
+    const int64_t slot = own_part_bytes(std::min(heads, group), a.head_size), ranges = int64_t(sms) * r.warps;
     r.own_at = up((items + sms) * r.tiles * int64_t(k.part_bytes));
     r.found_at = r.own_at + up((tail_items + ranges) * slot);
     r.bytes = r.found_at + up(tail_items * 8) + 256;

@@ -734,7 +734,8 @@ __global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(
   const unsigned tile = seq / unsigned(p.pre.tokens), grp = p.pre.turns ? tile : tile / unsigned(p.pre.tiles);
   const unsigned it = kvh * unsigned(p.pre.groups) + grp, u0 = it * unsigned(p.pre.key_tiles);
   const int row = int(seq - tile * p.pre.tokens) * p.group + hg * HPI;
-  const int64_t own_slot = int64_t(HPI) * (D * 4 + 8), part = 128 * (D * 4 + 8);
+  const unsigned room = min(HPI, unsigned(p.group));
+  const int64_t own_slot = own_part_bytes(room, D), part = 128 * (D * 4 + 8);
   grid_dependency();
   const unsigned cut = __ldcg(p.cut);
   int2 found = __ldcg(p.pre.found + item);
@@ -758,8 +759,8 @@ __global__ void __launch_bounds__(kCombineThreads) shared_prefix_combine_kernel(
     for (int k = 0; k < 4; ++k) {
       const int s = min(k0 + k * share, n - 1);
       const unsigned char* q = s < np ? own + s * own_slot : first + (s - np) * step;
-      ml[k] = __ldcg(reinterpret_cast<const float2*>(s < np ? q + HPI * D * 4 + hl * 8 : q + 128 * D * 4 + (row + hl) * 8));
-      v[k] = __ldcg(reinterpret_cast<const float4*>(s < np ? q + (d4 * HPI + hl) * 16 : q + (d4 * 128 + row + hl) * 16));
+      ml[k] = __ldcg(reinterpret_cast<const float2*>(s < np ? q + room * D * 4 + hl * 8 : q + 128 * D * 4 + (row + hl) * 8));
+      v[k] = __ldcg(reinterpret_cast<const float4*>(s < np ? q + (d4 * room + hl) * 16 : q + (d4 * 128 + row + hl) * 16));
       if (k0 + k * share >= n) ml[k] = make_float2(-INFINITY, 0.f);
     }
     float m_new = m;
