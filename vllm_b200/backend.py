@@ -85,7 +85,8 @@ class B200PagedAttentionMetadataBuilder:
     ``CommonAttentionMetadata`` (``utils.py:53-95``) does.
     """
 
-    # the ops neither allocate nor synchronise, so decode steps may be captured in full graphs
+    # the ops do not synchronise, and what a step allocates (v2's scratch, a shared prefix's) comes from the caching
+    # allocator, which takes part in a capture: decode steps may be captured in full graphs
     # (the reference spells this AttentionCGSupport.ALWAYS; the name is kept as a string so that
     # this module does not have to import vLLM)
     _cudagraph_support = "ALWAYS"

@@ -49,7 +49,8 @@ struct RotaryParams {
 
 __device__ __forceinline__ float nan_f32() { return __int_as_float(0x7fffffff); }
 
-// Every type, size, stride and alignment: a CTA to a token, a thread to a pair.
+// Every type, size, stride and alignment: a CTA to a token, a thread to a pair.  8192 tokens of 32 / 8 heads of 96, 24
+// dimensions rotated, bf16, 148 us (HBM alone 23), 32 / 32 heads of 80, 20 rotated, 278 (38), fp32 heads of 128 156 (62).
 template <typename in_t, typename cache_t, int KV>
 __global__ void __launch_bounds__(256) rotary_write_plain_kernel(const RotaryParams p) {
   grid_dependency_wait();
@@ -147,10 +148,12 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
 //     memory (ldmatrix.trans gives a lane four tokens of a dimension).  Tiles are moved onto 16-slot boundaries of
 //     the cache as in the other KV write kernels (kv_write_windows.h).
 // Measured on B200: 8192 tokens of 32 / 8 heads of 128, bf16, 42 us (4.9 TB/s of the 206 MB that it has to move); 16384
-// of 64 / 8 heads to fp8, chunks that start anywhere, 123 (5.2 TB/s; 139 with 24 warps to an SM and eight chunks a
-// thread, 24 and six 129, 16 and sixteen 141, 32 and eight, which spill, 152); flash layout, neighbours, a quarter
-// rotated, to e5m2, 47 (5.3).  The next heads' chunks on their way under the ones in work need registers that are
-// not there (spills: 47 -> 57).  What is left is latency: a warp loads, waits, turns and stores.
+// of 64 / 8 heads to fp8, chunks that start anywhere, 122 (5.3 TB/s; 139 with 24 warps to an SM and eight chunks a
+// thread, 24 and six 129, 16 and sixteen 141, 32 and eight 152); flash layout, neighbours, a quarter rotated, to e5m2,
+// 47 (5.3).  32 warps leave 64 registers, of which all twelve instantiations spill: 20 to 88 bytes a thread stored, up
+// to 116 loaded.  24 warps with eight chunks store 0 to 56 and are slower, 32 with eight up to 224.  With the next heads'
+// chunks on their way under the ones in work: 47 -> 57.  What is left is latency (a warp loads, waits, turns and
+// stores) and, for a step of 8192 tokens, 2560 unequal blocks on 592 places: 4.3 waves.
 template <typename in_t, int KV, bool kHalves>
 __global__ void __launch_bounds__(kRotaryThreads, 4) rotary_write_kernel(const RotaryParams p, const RotaryPlan plan) {
   using cache_t = std::conditional_t<KV == kKvAuto, in_t, uint8_t>;
