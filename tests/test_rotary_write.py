@@ -374,6 +374,17 @@ def test_the_c_interface_refuses_a_query_out_over_its_inputs(out, stride):
     assert capi.launch_count() == 0
 
 
+@pytest.mark.parametrize("stride", [0, 511, -512])
+def test_the_c_interface_refuses_rows_of_query_out_over_each_other(stride):
+    r, a, _ = _c_args(query_out_stride=stride, query_stride=stride)
+    a.key = a.value = r.query + 65536
+    with pytest.raises(RuntimeError, match="must not overlap"):
+        capi.rotary_reshape_and_cache(r, a)
+    a.num_tokens, a.key_cache = 1, None  # (one row: the stride means nothing; refused for the cache, not launched)
+    with pytest.raises(RuntimeError, match="null tensor"):
+        capi.rotary_reshape_and_cache(r, a)
+
+
 @pytest.mark.gpu
 def test_outputs_beside_the_inputs():
     """query_out in the same buffer as the projection's output, in columns of its own: no overlap."""

@@ -523,6 +523,7 @@ static int rotary_entry(const b200pa_rotary_args* r, const b200pa_cache_args* a,
   B200PA_CHECK_ARG(a->kv_dtype == B200PA_KV_AUTO || (a->k_scale && a->v_scale), "fp8 kv cache needs k_scale and v_scale");
   const int64_t es = a->in_dtype == B200PA_F32 ? 4 : 2, n = a->num_tokens, q_row = int64_t(r->num_heads) * a->head_size * es,
                 kv_row = int64_t(a->num_heads) * a->head_size * es;
+  B200PA_CHECK_ARG(n == 1 || r->query_out_stride * es >= q_row, "the rows of query_out must not overlap");
   const RowSpan out{r->query_out, r->query_out_stride * es, q_row};
   const bool in_place = r->query_out == r->query && (n == 1 || r->query_out_stride == r->query_stride);
   B200PA_CHECK_ARG((in_place || !rows_meet(out, {r->query, r->query_stride * es, q_row}, n)) &&
