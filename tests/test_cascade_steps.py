@@ -253,6 +253,35 @@ def test_a_cascade_is_one_native_call(monkeypatch, new, write):
     assert (out[0][n:] == 7.0).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("new", [[1] * 40, [1] * 40 + [30, 200]], ids=["decodes", "chunks"])
+def test_without_memory_for_the_scratch_a_cascade_is_an_ordinary_step(new):
+    """An engine may have given all device memory to its cache: the step then shares nothing and raises nothing."""
+    s = Session(len(new), 2048, [5 + 3 * i for i in range(len(new))])
+    md = s.step(new)
+    n = md.num_actual_tokens
+    q = torch.randn((n, s.H, s.D), generator=s.g).to(s.dtype).to(DEV)
+    out = [torch.empty((n, s.H * s.D), dtype=s.dtype, device=DEV) for _ in range(2)]
+    md.use_cascade = False
+    s.impl.forward(s.layer, q, None, None, s.cache, md, output=out[0])
+    md.use_cascade = True
+    torch.cuda.empty_cache()
+    hold = []  # what is free inside the allocator's segments, down to less than any scratch
+    torch.cuda.set_per_process_memory_fraction(1e-6)
+    for size in (1 << 26, 1 << 23, 1 << 21, (1 << 20) + 1):
+        try:
+            while True:
+                hold.append(torch.empty(size, dtype=torch.uint8, device=DEV))
+        except torch.OutOfMemoryError:
+            pass
+    try:
+        s.impl.forward(s.layer, q, None, None, s.cache, md, output=out[1])
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    torch.cuda.synchronize()
+    assert torch.equal(*out)
+
+
 def test_the_step_is_told_the_prefix(monkeypatch):
     seen = []
     monkeypatch.setattr(ops, "attention_step", lambda *a: seen.append(a[-1]) or True)

@@ -1026,9 +1026,14 @@ PyObject* py_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
       const int32_t length = static_cast<int32_t>(std::min<int64_t>(prefix, INT32_MAX));
       int32_t way = 0;
       if (b200pa_shared_prefix_route(&d, length, &way) != B200PA_OK) return false;
-      if (way != 0) {
-        const int64_t bytes = b200pa_shared_prefix_scratch_bytes(&d, length);
-        const at::Tensor scratch = at::empty({bytes}, q.options().dtype(ScalarType::Byte));
+      const int64_t bytes = way != 0 ? b200pa_shared_prefix_scratch_bytes(&d, length) : 0;
+      at::Tensor scratch;
+      try {
+        if (bytes > 0) scratch = at::empty({bytes}, q.options().dtype(ScalarType::Byte));
+      } catch (const c10::OutOfMemoryError&) {  // (an engine may have given all memory to its cache: an ordinary step)
+        (void)cudaGetLastError();
+      }
+      if (scratch.defined()) {
         if (write) check_rc(b200pa_reshape_and_cache(&c, stream));
         check_rc(b200pa_paged_attention_shared_prefix(&d, length, scratch.data_ptr(), bytes, stream));
         if (max_q == 1 || decodes >= reqs) return true;
