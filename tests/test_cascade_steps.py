@@ -282,8 +282,29 @@ def test_without_memory_for_the_scratch_a_cascade_is_an_ordinary_step(new):
     assert torch.equal(*out)
 
 
+@pytest.mark.gpu
+def test_a_captured_step_holds_for_batches_without_the_prefix():
+    """What is replayed may be any batch of as many decodes: a common prefix at capture says nothing about it."""
+    s = Session(40, 2048, [5 + 3 * i for i in range(40)])
+    md = s.step([1] * 40)
+    assert md.use_cascade
+    q = torch.randn((40, s.H, s.D), generator=s.g).to(s.dtype).to(DEV)
+    out, want = (torch.empty((40, s.H * s.D), dtype=s.dtype, device=DEV) for _ in range(2))
+    s.impl.forward(s.layer, q, None, None, s.cache, md, output=out)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        s.impl.forward(s.layer, q, None, None, s.cache, md, output=out)
+    md.block_table.copy_(torch.randint(0, s.nb, md.block_table.shape, generator=s.g).int())
+    md.use_cascade = False
+    s.impl.forward(s.layer, q, None, None, s.cache, md, output=want)
+    g.replay()
+    torch.cuda.synchronize()
+    assert (out.float() - want.float()).norm() <= 2e-2 * want.float().norm()
+
+
 def test_the_step_is_told_the_prefix(monkeypatch):
     seen = []
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
     monkeypatch.setattr(ops, "attention_step", lambda *a: seen.append(a[-1]) or True)
     impl = B200PagedAttentionImpl(8, 128, 0.1, 2)
     q, out = torch.zeros(3, 8, 128), torch.zeros(3, 1024)
@@ -295,3 +316,6 @@ def test_the_step_is_told_the_prefix(monkeypatch):
     for prefix in (64, 0):
         impl.forward(layer, q, None, None, torch.zeros(2, 6, 4096), b.build(prefix, common), output=out)
     assert seen == [64, 0]
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    impl.forward(layer, q, None, None, torch.zeros(2, 6, 4096), b.build(64, common), output=out)
+    assert seen == [64, 0, 0]

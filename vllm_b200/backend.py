@@ -203,11 +203,14 @@ class B200PagedAttentionImpl:
             alibi = self.alibi_slopes = alibi.to(query.device)
         # A captured step is replayed with other batches of its token count: what is cut off by a host
         # number at capture must hold for all of them.  The prefill kernel divides the step by the
-        # offsets and lengths on the device, single tokens among them.
-        num_decodes = md.num_decodes
-        if md.max_query_len > 1 and torch.cuda.is_current_stream_capturing():
-            num_decodes = 0
-        cascade = md.use_cascade and num_decodes > 1
+        # offsets and lengths on the device, single tokens among them; a common prefix would be the
+        # captured batch's.
+        num_decodes, cascade = md.num_decodes, md.use_cascade
+        if (cascade or md.max_query_len > 1) and torch.cuda.is_current_stream_capturing():
+            cascade = False
+            if md.max_query_len > 1:
+                num_decodes = 0
+        cascade = cascade and num_decodes > 1
         # (whether the decodes share the prefix in fact is decided there, by the sizes of the batch)
         if ops.attention_step(
                 output, query, key, value, kv_cache, md.block_table, md.seq_lens, md.slot_mapping,
